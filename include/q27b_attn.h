@@ -45,6 +45,8 @@ extern "C" {
 #define Q27B_MAX_T 4
 #define Q27B_PART_ROW 258 /* floats of one partial row: max, sum, unnormalised O[256] (src/attn.cu:26) */
 #define Q27B_PAGE 256     /* positions per page of the paged cache */
+#define Q27B_BLOCK 64     /* positions per block of the block-sparse operators */
+#define Q27B_MAX_TREE_T 64 /* drafted tokens of a tree */
 
 /* Text of the last error on this thread ("" if none). */
 const char* q27b_last_error(void);
@@ -423,6 +425,81 @@ int q27b_attn_prefill_q8_1(const float* qn, const float* qg, const void* kcache,
  * (the per-32-block accumulators of src/attn.cu:690-691, which must be bit-exact). */
 int q27b_prefill_qk_debug(const float* x, int rows, float kq_scale, const void* kcache, int nkvh, int n_ctx, int kh,
                           int p0, int npos, int8_t* q_i8, float* q_scale, int32_t* acc, void* stream);
+
+/* ---- Speculative decoding with a tree of drafts, and drafting with attention over few blocks of the cache.
+ * The reference verifies a chain of up to 4 drafts (src/model.cu:721-730) and reads the whole cache for each of its steps;
+ * these operators are new. A step of a tree of T drafts: q27b_attn_prep appends the T rows in the order of the drafts
+ * (rope3[t] = pos0 + depth[t], three times), q27b_attn_decode_tree attends, the caller samples and finds the accepted path,
+ * q27b_kv_commit moves its rows to the front, q27b_kv_bounds brings the blocks' bounds up to date. A draft step with few
+ * blocks: q27b_attn_prep, q27b_kv_bounds, q27b_select_blocks, q27b_attn_decode_blocks.
+ * All of them keep their scratch in the workspace: one stream order per device, as for the other entry points. Indices that
+ * the device finds out of range are skipped and reported in the device status word (bit 1: page table, bit 2: path or list
+ * of blocks). */
+
+/* Masks and depths of a tree of T = 1..64 drafts in which parent[t] is the draft before t (smaller than t) or -1 for a
+ * child of the last accepted token: mask[t] has bit j set for j = t and every ancestor j of t, depth[t] (may be null)
+ * counts the ancestors. Host only. */
+int q27b_tree_plan(const int* parent, int T, uint64_t* mask, int* depth);
+
+/* Attention of T = 1..64 drafts in cache rows *pos0 .. *pos0 + T - 1. Draft t sees the rows before *pos0 and those rows
+ * *pos0 + j for which bit j of mask[t] is set (its own only if bit t is; bits from T on are ignored); what the other rows
+ * hold has no influence. Otherwise as q27b_attn_decode: GQA 6:1, softmax, o *= sigmoid(gate); a draft that sees nothing
+ * gives 0. mask is device memory. Q * kq_scale, K, V and P are rounded to f16 for the tensor cores, sums are f32; the
+ * output is therefore f16 (o: __half [T][nqh][256]) or, with xq != null, q8_1 as in q27b_attn_decode. Partials lie in
+ * the prefill workspace. */
+int q27b_attn_decode_tree(const float* qn, const float* qg, const void* kcache, const void* vcache, void* o, int8_t* xq,
+                          float* xd, const int* pos0, const uint64_t* mask, int T, float kq_scale, int nqh, int nkvh,
+                          int n_ctx, int q8, void* stream);
+/* The same for B sequences over the page pool: T drafts each at positions seq_len[b] - T + t (seq_len counts them),
+ * mask [B][T]. max_seq_len: no seq_len[b] is larger (a longer one is cut there). Sequences with fewer drafts give the rows
+ * they do not use a mask of 0 and name them in no other: what such rows hold does not matter. B * T <= 65535. Partials lie
+ * in the paged workspace. */
+int q27b_attn_decode_tree_paged(const float* qn, const float* qg, const void* kpool, const void* vpool,
+                                const int* page_table, const int* seq_len, const uint64_t* mask, void* o, int8_t* xq,
+                                float* xd, int B, int T, float kq_scale, int nqh, int nkvh, int n_pages, int max_pages,
+                                int max_seq_len, void* stream);
+
+/* After verification: cache rows *pos0 + i <- *pos0 + path[i] for i < *count, every head, K and V (path int32 [T], count
+ * int32 [1], both on the device; T = 1..64 as in the tree call). All rows are read before any is written, so a path may
+ * name rows in any order; it usually ascends. An entry outside [0, T) leaves its row as it is and sets status bit 2;
+ * count is cut to [0, T]. The paged form: path [B][T], count [B], rows seq_len[b] - T + i. */
+int q27b_kv_commit(void* kcache, void* vcache, const int* pos0, const int* path, const int* count, int T, int nkvh,
+                   int n_ctx, int q8, void* stream);
+int q27b_kv_commit_paged(void* kpool, void* vpool, const int* page_table, const int* seq_len, const int* path,
+                         const int* count, int B, int T, int nkvh, int n_pages, int max_pages, void* stream);
+
+/* Bounds of the keys: for every block of 64 positions, head and dim the smallest and the largest value of K as attention
+ * reads it (f16; q8_0: value times scale). Layout f16 [nkvh][ceil(n_ctx / 64)][2][256] beside a contiguous cache,
+ * [n_pages][nkvh][4][2][256] beside a K pool. The call writes the bounds of every block that holds one of the rows
+ * *pos0 .. *pos0 + T - 1 (paged: seq_len[b] - T ..), over all rows of the block below *pos0 + T: after an append, a commit
+ * or a prompt's chunk, or of the whole cache at once. NaN in a key makes its bound NaN. */
+uint64_t q27b_kv_bounds_bytes(int nkvh, int n_ctx);
+uint64_t q27b_kv_bounds_pool_bytes(int nkvh, int n_pages);
+int q27b_kv_bounds(const void* kcache, void* bounds, const int* pos0, int T, int nkvh, int n_ctx, int q8, void* stream);
+int q27b_kv_bounds_paged(const void* kpool, void* bounds, const int* page_table, const int* seq_len, int B, int T, int nkvh,
+                         int n_pages, int max_pages, void* stream);
+
+/* Which blocks each of T = 1..4 tokens at positions *pos0 + t attends, for every KV head: of the blocks up to the token's
+ * own the first n_sink and the last n_recent (>= 1) always, and of the others those of the highest score, k in all.
+ * score = max over the KV head's six query heads of sum_d max(q_d lo_d, q_d hi_d), an upper bound of q.k over the block,
+ * summed in 64 bits; of equal scores the lower block wins, NaN wins over everything. sel int32 [T][nkvh][k] ascending,
+ * -1 behind the last block when the token has fewer than k. At most 1,048,576 positions; n_sink + n_recent <= k. */
+int q27b_select_blocks(const float* qn, const void* bounds, int* sel, const int* pos0, int T, int k, int n_sink,
+                       int n_recent, int nqh, int nkvh, int n_ctx, void* stream);
+int q27b_select_blocks_paged(const float* qn, const void* bounds, int* sel, const int* page_table, const int* seq_len,
+                             int B, int T, int k, int n_sink, int n_recent, int nqh, int nkvh, int n_pages, int max_pages,
+                             int max_seq_len, void* stream);
+
+/* q27b_attn_decode in which token t reads, for KV head h, only the blocks sel[t][h][0..k) (k <= 16384), up to its own
+ * position *pos0 + t. -1 stands for no block; an entry below -1 or behind the cache is skipped and sets status bit 2; a block
+ * that is named twice counts twice. A token without a visible row gives 0. Output as in q27b_attn_decode_tree. */
+int q27b_attn_decode_blocks(const float* qn, const float* qg, const void* kcache, const void* vcache, void* o, int8_t* xq,
+                            float* xd, const int* pos0, const int* sel, int T, int k, float kq_scale, int nqh, int nkvh,
+                            int n_ctx, int q8, void* stream);
+int q27b_attn_decode_blocks_paged(const float* qn, const float* qg, const void* kpool, const void* vpool,
+                                  const int* page_table, const int* seq_len, const int* sel, void* o, int8_t* xq, float* xd,
+                                  int B, int T, int k, float kq_scale, int nqh, int nkvh, int n_pages, int max_pages,
+                                  void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,8 +23,10 @@ LIB_PATH = os.environ.get("Q27B_LIB") or os.path.join(_HERE, "libq27b_attn.so")
 HEAD_DIM = 256
 GQA = 6
 MAX_T = 4
+MAX_TREE_T = 64
 PART_ROW = 258
 PAGE = 256
+BLOCK = 64
 
 OK, BAD_SHAPE, CUDA_ERROR, UNSUPPORTED, DEVICE_STATUS = 0, 1, 2, 3, 4
 
@@ -42,6 +44,9 @@ SYMBOLS = [
     "q27b_attn_prep_paged", "q27b_pager_create", "q27b_pager_destroy", "q27b_pager_open", "q27b_pager_extend",
     "q27b_pager_cut", "q27b_pager_close", "q27b_pager_fork", "q27b_pager_free_pages", "q27b_pager_len",
     "q27b_pager_tables", "q27b_kv_page_copy", "q27b_pager_unshare", "q27b_attn_decode_exchange", "q27b_sum_exchange_norm_q8",
+    "q27b_tree_plan", "q27b_attn_decode_tree", "q27b_attn_decode_tree_paged", "q27b_kv_commit", "q27b_kv_commit_paged",
+    "q27b_kv_bounds_bytes", "q27b_kv_bounds_pool_bytes", "q27b_kv_bounds", "q27b_kv_bounds_paged", "q27b_select_blocks",
+    "q27b_select_blocks_paged", "q27b_attn_decode_blocks", "q27b_attn_decode_blocks_paged",
 ]
 
 
@@ -56,6 +61,8 @@ def _load():
     lib.q27b_kv_wire_bytes.restype = ctypes.c_uint64
     lib.q27b_xbuf_bytes.restype = ctypes.c_uint64
     lib.q27b_sum_xbuf_bytes.restype = ctypes.c_uint64
+    lib.q27b_kv_bounds_bytes.restype = ctypes.c_uint64
+    lib.q27b_kv_bounds_pool_bytes.restype = ctypes.c_uint64
     lib.q27b_pager_destroy.restype = None
     lib.q27b_pager_destroy.argtypes = [ctypes.c_void_p]
     return lib
@@ -75,7 +82,9 @@ def _check(rc):
         raise Q27Error(rc, _lib.q27b_last_error().decode())
 
 
-def _ptr(t, dtype=None, optional=False):
+def _ptr(t, dtype=None, optional=False, least=0):
+    """Device address of a tensor argument; least > 0: it must lie on the current device and have that many elements
+    (dtype None: bytes)."""
     if isinstance(t, int):  # a raw device address (exchange buffers mapped from other processes)
         return ctypes.c_void_p(t)
     if t is None:
@@ -86,6 +95,12 @@ def _ptr(t, dtype=None, optional=False):
         raise Q27Error(BAD_SHAPE, "tensors must be contiguous CUDA tensors")
     if dtype is not None and t.dtype != dtype:
         raise Q27Error(BAD_SHAPE, "expected dtype %s, got %s" % (dtype, t.dtype))
+    if least > 0:
+        have = t.numel() * (t.element_size() if dtype is None else 1)
+        if have < least:
+            raise Q27Error(BAD_SHAPE, "expected at least %d %s, got %d" % (least, "bytes" if dtype is None else "elements", have))
+        if t.get_device() != torch.cuda.current_device():
+            raise Q27Error(BAD_SHAPE, "a tensor lies on cuda:%d, the current device is cuda:%d" % (t.get_device(), torch.cuda.current_device()))
     return ctypes.c_void_p(t.data_ptr())
 
 
@@ -114,8 +129,11 @@ def _load_binding():
     mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("q27b_binding", loader))
     loader.exec_module(mod)
     fns = tuple(ctypes.cast(getattr(_lib, "q27b_" + n), ctypes.c_void_p).value
-                for n in ("attn_prep", "attn_decode", "attn_prep_paged", "attn_decode_paged", "attn_prefill"))
-    mod.bind(fns, _ptr, _check, torch.float32, torch.int32, torch.int8)
+                for n in ("attn_prep", "attn_decode", "attn_prep_paged", "attn_decode_paged", "attn_prefill",
+                          "attn_decode_tree", "attn_decode_tree_paged", "kv_commit", "kv_commit_paged", "kv_bounds",
+                          "kv_bounds_paged", "select_blocks", "select_blocks_paged", "attn_decode_blocks",
+                          "attn_decode_blocks_paged"))
+    mod.bind(fns, _ptr, _check, torch.float32, torch.int32, torch.int8, torch.float16, torch.int64)
     return mod
 
 
@@ -434,6 +452,85 @@ def attn_prep_paged(qg, k, v, q_norm, k_norm, qn, kpool, vpool, page_table, seq_
     """q27::attn_prep for B sequences over the page pool; with q_norm None it only appends K and V."""
     _native.attn_prep_paged(qg, k, v, q_norm, k_norm, qn, kpool, vpool, page_table, seq_len, B, T, eps, theta_scale, nqh,
                             nkvh, n_pages, max_pages, rope3, rdelta)
+
+
+# ---- trees of drafts, and attention over few blocks of the cache
+def tree_plan(parent):
+    """(mask int64 [T], depth int32 [T]) as numpy arrays for a tree of T = 1..64 drafts: parent[t] is the draft before t, or
+    -1 behind the last accepted token. The mask goes to attn_decode_tree (as a CUDA tensor), pos0 + depth into rope3."""
+    import numpy as np
+    T = len(parent)
+    par = (ctypes.c_int * max(T, 1))(*[int(x) for x in parent])
+    mask, depth = np.zeros((T,), np.int64), np.zeros((T,), np.int32)
+    _check(_lib.q27b_tree_plan(par, T, mask.ctypes.data_as(ctypes.c_void_p), depth.ctypes.data_as(ctypes.c_void_p)))
+    return mask, depth
+
+
+def attn_decode_tree(qn, qg, kcache, vcache, o, xq, xd, pos0, mask, T, kq_scale, nqh, nkvh, n_ctx, q8=True):
+    """Attention of T = 1..64 drafts in rows *pos0 + t: draft t sees the rows before *pos0 and the drafts of mask[t] (int64).
+    o: f16 [T][nqh][256]; with xq given the result goes to q8_1 (xq, xd) instead."""
+    _native.attn_decode_tree(qn, qg, kcache, vcache, o, xq, xd, pos0, mask, T, kq_scale, nqh, nkvh, n_ctx, q8)
+
+
+def attn_decode_tree_paged(qn, qg, kpool, vpool, page_table, seq_len, mask, o, xq, xd, B, T, kq_scale, nqh, nkvh, n_pages,
+                           max_pages, max_seq_len):
+    """attn_decode_tree for B sequences over the page pool (mask [B][T], drafts at positions seq_len[b] - T + t)."""
+    _native.attn_decode_tree_paged(qn, qg, kpool, vpool, page_table, seq_len, mask, o, xq, xd, B, T, kq_scale, nqh, nkvh,
+                                   n_pages, max_pages, max_seq_len)
+
+
+def kv_commit(kcache, vcache, pos0, path, count, T, nkvh, n_ctx, q8=True):
+    """Rows *pos0 + i <- *pos0 + path[i], i < *count (int32, on the device): the accepted path of a tree of T drafts."""
+    _native.kv_commit(kcache, vcache, pos0, path, count, T, nkvh, n_ctx, q8)
+
+
+def kv_commit_paged(kpool, vpool, page_table, seq_len, path, count, B, T, nkvh, n_pages, max_pages):
+    """kv_commit for B sequences over the page pool (path [B][T], count [B], rows seq_len[b] - T + i)."""
+    _native.kv_commit_paged(kpool, vpool, page_table, seq_len, path, count, B, T, nkvh, n_pages, max_pages)
+
+
+def kv_bounds_bytes(nkvh, n_ctx):
+    """Bytes of the block bounds of one K cache: f16 [nkvh][ceil(n_ctx / 64)][2][256]."""
+    return int(_lib.q27b_kv_bounds_bytes(int(nkvh), int(n_ctx)))
+
+
+def kv_bounds_pool_bytes(nkvh, n_pages):
+    """Bytes of the block bounds of one K pool: f16 [n_pages][nkvh][4][2][256]."""
+    return int(_lib.q27b_kv_bounds_pool_bytes(int(nkvh), int(n_pages)))
+
+
+def kv_bounds(kcache, bounds, pos0, T, nkvh, n_ctx, q8=True):
+    """Smallest and largest key per dim of every 64-row block that holds one of the rows *pos0 .. *pos0 + T - 1."""
+    _native.kv_bounds(kcache, bounds, pos0, T, nkvh, n_ctx, q8)
+
+
+def kv_bounds_paged(kpool, bounds, page_table, seq_len, B, T, nkvh, n_pages, max_pages):
+    """kv_bounds for the last T rows of B sequences over the page pool."""
+    _native.kv_bounds_paged(kpool, bounds, page_table, seq_len, B, T, nkvh, n_pages, max_pages)
+
+
+def select_blocks(qn, bounds, sel, pos0, T, k, n_sink, n_recent, nqh, nkvh, n_ctx):
+    """sel int32 [T][nkvh][k]: the blocks that each of T = 1..4 tokens attends per KV head, ascending, -1 behind the last."""
+    _native.select_blocks(qn, bounds, sel, pos0, T, k, n_sink, n_recent, nqh, nkvh, n_ctx)
+
+
+def select_blocks_paged(qn, bounds, sel, page_table, seq_len, B, T, k, n_sink, n_recent, nqh, nkvh, n_pages, max_pages,
+                        max_seq_len):
+    """select_blocks for B sequences over the page pool (sel [B][T][nkvh][k])."""
+    _native.select_blocks_paged(qn, bounds, sel, page_table, seq_len, B, T, k, n_sink, n_recent, nqh, nkvh, n_pages, max_pages,
+                                max_seq_len)
+
+
+def attn_decode_blocks(qn, qg, kcache, vcache, o, xq, xd, pos0, sel, T, k, kq_scale, nqh, nkvh, n_ctx, q8=True):
+    """attn_decode of T = 1..4 tokens over the blocks of sel only, up to each token's own position; o: f16, or q8_1."""
+    _native.attn_decode_blocks(qn, qg, kcache, vcache, o, xq, xd, pos0, sel, T, k, kq_scale, nqh, nkvh, n_ctx, q8)
+
+
+def attn_decode_blocks_paged(qn, qg, kpool, vpool, page_table, seq_len, sel, o, xq, xd, B, T, k, kq_scale, nqh, nkvh, n_pages,
+                             max_pages):
+    """attn_decode_blocks for B sequences over the page pool."""
+    _native.attn_decode_blocks_paged(qn, qg, kpool, vpool, page_table, seq_len, sel, o, xq, xd, B, T, k, kq_scale, nqh, nkvh,
+                                     n_pages, max_pages)
 
 
 def kv_page_copy(pool, src_page, dst_page, rows, nkvh, n_pages):

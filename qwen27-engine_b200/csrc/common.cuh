@@ -19,6 +19,7 @@ constexpr float LOG2E = 1.4426950408889634f;
 // Bits of the per-device status word written by kernels.
 constexpr int ST_WAIT_EXPIRED = 1;   // a bounded mbarrier wait gave up
 constexpr int ST_BAD_PAGE = 2;       // a page-table entry was out of range (the page was skipped)
+constexpr int ST_BAD_INDEX = 4;      // an entry of a path or of a list of blocks was out of range (it was skipped)
 
 // The reference's kernels all start with these two (src/common.cuh:17-21), so that they stay
 // legal under its programmatic-dependent launches.
