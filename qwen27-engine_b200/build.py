@@ -15,7 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(HERE, "build")
 LIB = os.path.join(HERE, "libq27b_attn.so")
-SOURCES = ["host.cu", "kv_append.cu", "kv_wire.cu", "kv_blocks.cu", "combine.cu", "decode.cu", "decode_tc.cu", "decode_ws.cu", "decode_wt.cu", "decode_ref.cu", "decode_rows.cu", "prefill.cu", "prefill_f16.cu", "sum_norm.cu", "peak_mma.cu", "pager.cu"]
+SOURCES = ["host.cu", "kv_append.cu", "kv_wire.cu", "kv_blocks.cu", "combine.cu", "decode.cu", "decode_tc.cu", "decode_ws.cu", "decode_wt.cu", "decode_ref.cu", "decode_rows.cu", "decode_tree.cu", "prefill.cu", "prefill_f16.cu", "sum_norm.cu", "peak_mma.cu", "pager.cu"]
 BINDING = os.path.join(HERE, "q27b_binding.so")
 BINDING_SOURCES = [os.path.join(CSRC, "binding.cpp"), os.path.join(HERE, "..", "include", "q27b_attn.h")]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

@@ -59,10 +59,10 @@ inline CacheRef paged_ref(const DeviceCtx* ctx, const int* page_table, const int
 }
 // Shape checks that the entry points share. Row and page counts stay within what an int holds.
 inline bool bad_contiguous(int T, int max_T, int nkvh, int n_ctx) {
-  return T < 1 || T > max_T || nkvh < 1 || nkvh > 65535 || n_ctx < 1 || (int64_t)nkvh * n_ctx > 0x7fffffff;
+  return T < 1 || T > max_T || nkvh < 1 || nkvh > 16384 || n_ctx < 1 || (int64_t)nkvh * n_ctx > 0x7fffffff;
 }
 inline bool bad_paged(int B, int T, int max_T, int nkvh, int n_pages, int max_pages) {
-  return B < 1 || B > 65535 || T < 1 || T > max_T || nkvh < 1 || nkvh > 65535 || n_pages < 1 || max_pages < 1 ||
+  return B < 1 || B > 65535 || T < 1 || T > max_T || nkvh < 1 || nkvh > 16384 || n_pages < 1 || max_pages < 1 ||
          max_pages > (1 << 22) || (int64_t)n_pages * nkvh * Q27B_PAGE > 0x7fffffff;
 }
 

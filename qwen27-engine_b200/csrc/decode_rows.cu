@@ -34,16 +34,15 @@ __device__ __forceinline__ void load8(const uint8_t* base, size_t scales, bool q
   }
 }
 
-__global__ void __launch_bounds__(32 * WARPS) rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(32 * WARPS) blocks_kernel(const RowsParams p) {
   __shared__ float sm[WARPS][GQA], sl[WARPS][GQA], so[WARPS][AD];
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int z = blockIdx.x, kh = blockIdx.y, b = blockIdx.z / p.c.T, t = blockIdx.z % p.c.T, nqh = p.c.nkvh * GQA;
   pdl_wait();
   const int first = first_pos(p.c, b), n = max(0, min(first + p.c.T, p.c.n_ctx));
-  const int ntiles = p.sel ? p.k : (n + BLK - 1) / BLK, share = (ntiles + p.nsplit - 1) / p.nsplit;
-  const uint64_t mask = p.sel ? 0 : p.mask[(size_t)b * p.c.T + t];
-  const int* list = p.sel ? p.sel + (((size_t)b * p.c.T + t) * p.c.nkvh + kh) * p.k : nullptr;
+  const int share = (p.k + p.nsplit - 1) / p.nsplit;
+  const int* list = p.sel + (((size_t)b * p.c.T + t) * p.c.nkvh + kh) * p.k;
   const size_t row0 = ((size_t)b * p.c.T + t) * nqh + kh * GQA;  // the first of the six output rows
   float q[GQA][8], o[GQA][8], m[GQA], l[GQA];
 #pragma unroll
@@ -55,22 +54,19 @@ __global__ void __launch_bounds__(32 * WARPS) rows_kernel(const RowsParams p) {
     l[g] = 0.f;
   }
   const size_t scales = cache_rows(p.c) * AD;
-  for (int i = z * share; i < min(ntiles, (z + 1) * share); i++) {
-    int tile = i;
-    if (list) {
-      tile = list[i];
-      if (tile == -1) continue;
-      if (tile < -1 || tile > (p.c.n_ctx - 1) / BLK) {
-        if (threadIdx.x == 0) atomicOr(p.c.status, ST_BAD_INDEX);
-        continue;
-      }
+  for (int i = z * share; i < min(p.k, (z + 1) * share); i++) {
+    const int tile = list[i];
+    if (tile == -1) continue;
+    if (tile < -1 || tile > (p.c.n_ctx - 1) / BLK) {
+      if (threadIdx.x == 0) atomicOr(p.c.status, ST_BAD_INDEX);
+      continue;
     }
     if (tile * BLK >= n) continue;
     const int64_t base = cache_row(p.c, b, kh, tile * BLK);
     if (base < 0) continue;
     for (int r = warp; r < BLK; r += WARPS) {
-      const int pos = tile * BLK + r, j = pos - first;
-      if (pos >= n || (list ? j > t : j >= 0 && !((mask >> j) & 1))) continue;
+      const int pos = tile * BLK + r;
+      if (pos >= n || pos > first + t) continue;
       float x[8], s[GQA];
       load8((const uint8_t*)p.kcache, scales, p.c.q8, base + r, lane, x);
 #pragma unroll
@@ -126,11 +122,16 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p) {
   pdl_wait();
   pdl_trigger();
   const float2* ml = p.part_ml + row * p.nsplit;
+  int np = p.nsplit;  // partials that were written
+  if (!p.sel) {
+    const int b = (int)(row / ((size_t)p.c.T * p.c.nkvh * GQA)), ntot = tree_tiles(min(first_pos(p.c, b) + p.c.T, p.c.n_ctx));
+    np = ntot ? (ntot - 1) / tree_share(p, ntot) + 1 : 0;
+  }
   float M = M_INIT;
-  for (int z = 0; z < p.nsplit; z++) M = fmaxf(M, ml[z].x);
+  for (int z = 0; z < np; z++) M = fmaxf(M, ml[z].x);
   float L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int z = grp; z < p.nsplit; z += 4) {
+  for (int z = grp; z < np; z += 4) {
     const float2 v = ml[z];
     if (v.y == 0.f) continue;  // holds nothing
     const float f = ex2((v.x - M) * LOG2E);
@@ -173,13 +174,12 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p) {
 // Rounds a workspace of `floats` down to the splits that it holds of `rows` rows.
 int64_t splits_that_fit(size_t floats, int64_t rows) { return (int64_t)(floats / ((size_t)rows * (AD + 2))); }
 
-int run_rows(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
-  const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, ctas = (int64_t)p.c.B * p.c.T * p.c.nkvh;
-  const int64_t tiles = p.sel ? p.k : (p.max_len + BLK - 1) / BLK;
-  int64_t ns = std::max<int64_t>(1, std::min<int64_t>({tiles, 64, (8 * (int64_t)ctx->n_sm + ctas - 1) / ctas}));
+// Partials of `rows` rows in *nsplit splits: in the prefill workspace, whose size is fixed (fewer splits where it holds no
+// more), or, for a batch, in the paged workspace.
+int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t nsplit, const char* who) {
   float* part;
   if (p.c.page_table) {
-    if (int rc = paged_ws(ctx, (size_t)rows * ns * (AD + 2), &part)) return rc;
+    if (int rc = paged_ws(ctx, (size_t)rows * nsplit * (AD + 2), &part)) return rc;
   } else {
     size_t cap;
     if (int rc = prefill_ws(ctx, &part, &cap)) return rc;
@@ -188,12 +188,38 @@ int run_rows(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
       return fail(Q27B_UNSUPPORTED, std::string(who) + ": the prefill workspace (" + std::to_string(cap * sizeof(float)) +
                                         " bytes) is too small for the partials of this call (" +
                                         std::to_string((size_t)rows * (AD + 2) * sizeof(float)) + " bytes)");
-    ns = std::min(ns, fit);
+    nsplit = std::min(nsplit, fit);
   }
-  p.nsplit = (int)ns;
+  p.nsplit = (int)nsplit;
   p.part_o = part;
-  p.part_ml = (float2*)(part + (size_t)rows * ns * AD);
-  Q27B_CK(launch_step(rows_kernel, dim3((unsigned)ns, p.c.nkvh, p.c.B * p.c.T), dim3(32 * WARPS), 0, s, p));
+  p.part_ml = (float2*)(part + (size_t)rows * nsplit * AD);
+  return Q27B_OK;
+}
+
+int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
+  const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, ctas = (int64_t)p.c.B * p.c.T * p.c.nkvh;
+  const int64_t ns = std::max<int64_t>(1, std::min<int64_t>({p.k, 64, (8 * (int64_t)ctx->n_sm + ctas - 1) / ctas}));
+  if (int rc = place_partials(ctx, p, rows, ns, who)) return rc;
+  Q27B_CK(launch_step(blocks_kernel, dim3(p.nsplit, p.c.nkvh, p.c.B * p.c.T), dim3(32 * WARPS), 0, s, p));
+  Q27B_CK(launch_step(rows_merge_kernel, dim3((unsigned)rows), dim3(256), 0, s, p));
+  return Q27B_OK;
+}
+
+// One sequence: a CTA per SM, the positions of every row tile in equal shares. A batch: shares of equal length, so that the
+// sequences' CTAs come to about four rounds of the SMs if all are of the largest length.
+int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
+  const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, ctas = (int64_t)p.c.B * p.c.nkvh * tree_row_tiles(p.c.T);
+  const int64_t tiles = tree_tiles(p.c.n_ctx);
+  int64_t ns;
+  if (p.c.page_table) {
+    const int64_t share = std::min<int64_t>(TREE_MAX_SHARE, std::max<int64_t>(8, ctas * tiles / (4 * ctx->n_sm)));
+    p.share = (int)share;
+    ns = (tiles + share - 1) / share;
+  } else {
+    ns = std::max<int64_t>(1, std::min(tiles, ctx->n_sm / ctas));
+  }
+  if (int rc = place_partials(ctx, p, rows, ns, who)) return rc;
+  if (int rc = launch_tree(p, s)) return rc;
   Q27B_CK(launch_step(rows_merge_kernel, dim3((unsigned)rows), dim3(256), 0, s, p));
   return Q27B_OK;
 }
@@ -233,8 +259,7 @@ int q27b_attn_decode_tree(const float* qn, const float* qg, const void* kcache, 
   RowsParams p = {};
   p.c = contiguous_ref(ctx, pos0, T, nkvh, n_ctx, q8);
   p.qn = qn; p.qg = qg; p.kcache = kcache; p.vcache = vcache; p.o = o; p.xq = xq; p.xd = xd; p.mask = mask; p.kq_scale = kq_scale;
-  p.max_len = n_ctx;
-  return run_rows(ctx, p, "attn_decode_tree", (cudaStream_t)stream);
+  return run_tree(ctx, p, "attn_decode_tree", (cudaStream_t)stream);
 }
 
 int q27b_attn_decode_tree_paged(const float* qn, const float* qg, const void* kpool, const void* vpool, const int* page_table,
@@ -251,8 +276,7 @@ int q27b_attn_decode_tree_paged(const float* qn, const float* qg, const void* kp
   p.c = paged_ref(ctx, page_table, seq_len, B, T, nkvh, n_pages, max_pages);
   p.c.n_ctx = max_seq_len;  // a longer sequence is cut there
   p.qn = qn; p.qg = qg; p.kcache = kpool; p.vcache = vpool; p.o = o; p.xq = xq; p.xd = xd; p.mask = mask; p.kq_scale = kq_scale;
-  p.max_len = max_seq_len;
-  return run_rows(ctx, p, "attn_decode_tree_paged", (cudaStream_t)stream);
+  return run_tree(ctx, p, "attn_decode_tree_paged", (cudaStream_t)stream);
 }
 
 int q27b_attn_decode_blocks(const float* qn, const float* qg, const void* kcache, const void* vcache, void* o, int8_t* xq,
@@ -267,8 +291,8 @@ int q27b_attn_decode_blocks(const float* qn, const float* qg, const void* kcache
   RowsParams p = {};
   p.c = contiguous_ref(ctx, pos0, T, nkvh, n_ctx, q8);
   p.qn = qn; p.qg = qg; p.kcache = kcache; p.vcache = vcache; p.o = o; p.xq = xq; p.xd = xd; p.sel = sel; p.k = k;
-  p.kq_scale = kq_scale; p.max_len = n_ctx;
-  return run_rows(ctx, p, "attn_decode_blocks", (cudaStream_t)stream);
+  p.kq_scale = kq_scale;
+  return run_blocks(ctx, p, "attn_decode_blocks", (cudaStream_t)stream);
 }
 
 int q27b_attn_decode_blocks_paged(const float* qn, const float* qg, const void* kpool, const void* vpool, const int* page_table,
@@ -284,8 +308,8 @@ int q27b_attn_decode_blocks_paged(const float* qn, const float* qg, const void* 
   RowsParams p = {};
   p.c = paged_ref(ctx, page_table, seq_len, B, T, nkvh, n_pages, max_pages);
   p.qn = qn; p.qg = qg; p.kcache = kpool; p.vcache = vpool; p.o = o; p.xq = xq; p.xd = xd; p.sel = sel; p.k = k;
-  p.kq_scale = kq_scale; p.max_len = max_pages * Q27B_PAGE;
-  return run_rows(ctx, p, "attn_decode_blocks_paged", (cudaStream_t)stream);
+  p.kq_scale = kq_scale;
+  return run_blocks(ctx, p, "attn_decode_blocks_paged", (cudaStream_t)stream);
 }
 
 }  // extern "C"

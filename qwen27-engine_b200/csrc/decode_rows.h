@@ -20,11 +20,20 @@ struct RowsParams {
   const uint64_t* mask;  // tree: [B][T], bit j: draft j is visible
   const int* sel;        // blocks: [B][T][nkvh][k], -1 = none; null: tree
   int k;
-  int max_len;           // no sequence is longer
   float kq_scale;
   int nsplit;
+  int share;             // tree, paged: position tiles of a split; 0: an equal share of the sequence's
   float* part_o;         // [row][nsplit][256], unnormalised
   float2* part_ml;       // [row][nsplit] (max, sum)
 };
+
+// The tensor-core kernel of the tree (decode_tree.cu): grid (splits, row tiles x KV heads, sequences).
+constexpr int TREE_ROWS = 128;       // (draft, head) rows of a KV head in a CTA
+constexpr int TREE_MAX_SHARE = 2048;  // position tiles of a split with pages
+__host__ __device__ inline int tree_row_tiles(int T) { return (T * GQA + TREE_ROWS - 1) / TREE_ROWS; }
+__host__ __device__ inline int tree_tiles(int n) { return n > 0 ? (n + BLK - 1) / BLK : 0; }
+// Tiles of a split of a sequence of ntot tiles; split z holds tiles z * share .. of them.
+__host__ __device__ inline int tree_share(const RowsParams& p, int ntot) { return p.share ? p.share : (ntot + p.nsplit - 1) / p.nsplit; }
+int launch_tree(const RowsParams& p, cudaStream_t s);
 
 }  // namespace q27b
