@@ -2,6 +2,7 @@
 // of the drafted rows (commit), per-block bounds of the keys (bounds), choice of the blocks to attend (select).
 #include "cache_ref.h"
 
+#include <algorithm>
 #include <mutex>
 
 namespace q27b {
@@ -161,27 +162,169 @@ int launch_bounds(const CacheRef& c, const void* kcache, void* bounds, cudaStrea
 }
 
 // ---------------------------------------------------------------- select
-// score(block) = max over the six query heads of the KV head of sum_d max(q_d lo_d, q_d hi_d): no key of the block has a
-// larger q.k. The order of scores decides what is attended, so they are sums in 64 bits (the products of f32 and f16
-// values are exact there): which block wins does not depend on the order of a sum, short of differences of 1e-16.
+// score(block) = max over the six query heads of the KV head of sum_d max(q_d lo_d, q_d hi_d) = sum_d (q+_d hi_d + q-_d lo_d):
+// no key of the block has a larger q.k. The order of scores decides what is attended, so it is that of sums in 64 bits,
+// in which the products of f32 and f16 values are exact: which block wins does not depend on the order of a sum, short of
+// differences of 1e-16. Two kernels:
+//  * score_kernel: every score to about 15 bits on the tensor cores, with a bound of its error;
+//  * select_kernel: what the bounds leave open around the border (a few blocks) again in 64 bits, and the choice.
+// All scores in 64 bits take ten times as long as reading the bounds (32 sequences of up to 131,072 positions, two tokens:
+// 222 us): two selects and an FMA at half rate per dim and head.
 struct SelectParams {
   CacheRef c;
   const float* qn;        // [B][T][6 nkvh][256]
   const __half* bounds;
   int* sel;               // [B][T][nkvh][k]
-  int k, n_sink, n_recent;
+  float2* score;          // [B][T][nkvh][max_blocks] (score, error)
+  int k, n_sink, n_recent, max_blocks;
 };
-constexpr int SEL_THREADS = 512;
 constexpr int SEL_MAX_BLOCKS = 16384;
 
-// Keys in the order of the scores: larger score, larger key; NaN above all.
-__device__ __forceinline__ unsigned long long score_key(double s) {
-  if (s != s) return ~0ull;
-  const long long bits = __double_as_longlong(s + 0.0);
-  return bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | 0x8000000000000000ull;
+// Blocks up to the own one of token t of sequence b.
+__device__ __forceinline__ int blocks_of(const CacheRef& c, int b, int t) {
+  const int last = min(first_pos(c, b) + t, c.n_ctx - 1);
+  return last < 0 ? 0 : last / BLK + 1;
 }
-// Exclusive sum over the block of x (two counts, 32 bits each); *total of all threads.
-__device__ __forceinline__ unsigned long long block_scan(unsigned long long x, unsigned long long* sums, unsigned long long* total) {
+
+// A warp scores 16 blocks of a (KV head, sequence) for all its tokens with m16n8k16 MMAs: the bounds are the A operand as they
+// lie in memory (a lane's 16 bytes are two k-steps; the order of the dims is free), all of them in registers at once, the
+// query heads are six of the eight columns of B. q times a power of two, so that its largest value is below 2^10, is the sum
+// of two f16 values, off by at most 2^-22 of itself or 2^-25. Three accumulators: q+ hi and q- lo with the larger parts, 16 MMAs
+// each, and both with the smaller parts. With A = sum |q| max(|lo|, |hi|) (a fourth one, of |q| + 2^-6), and 17 addends of
+// an MMA each cut at 2^-23 of the largest, the error is below 16 * 18 * 2^-23 A + 2^-22 A < 2^-14.7 A; 2^-14 A is what is
+// passed on. Bound by reading the bounds once they fill the SMs.
+constexpr int SCORE_WARPS = 4, SCORE_GROUP = 16 * SCORE_WARPS, Q_STRIDE = 2 * AD + 64;  // bytes between staged query rows: 16-byte reads without conflicts
+enum { QP_HI, QM_HI, QP_LO, QM_LO, QABS, Q_PARTS };
+constexpr int Q_TOKEN = Q_PARTS * 8 * Q_STRIDE;  // bytes of a staged token
+
+__global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const SelectParams p) {
+  extern __shared__ __align__(16) uint8_t sq[];  // [T][Q_PARTS][8 columns][Q_STRIDE]
+  __shared__ float unit[Q27B_MAX_T][8];          // 1 / scale of a head
+  pdl_trigger();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
+  const int kh = blockIdx.y, b = blockIdx.z, T = p.c.T, nqh = p.c.nkvh * GQA;
+  for (int i = tid; i < T * Q_PARTS * 2 * Q_STRIDE / 4; i += 32 * SCORE_WARPS)  // the two columns that are no head
+    *(uint32_t*)&sq[i / (2 * Q_STRIDE / 4) * (8 * Q_STRIDE) + 6 * Q_STRIDE + i % (2 * Q_STRIDE / 4) * 4] = 0;
+  pdl_wait();
+  const int nb = blocks_of(p.c, b, T - 1), ngroups = (nb + SCORE_GROUP - 1) / SCORE_GROUP;
+  if (nb <= p.k || (int)blockIdx.x >= ngroups) return;  // every block is taken; or no block of this sequence
+  uint4 lo[2][8], hi[2][8];  // rows g and g + 8, 32 dims each: 8 of them in this lane
+  bool there[2];
+  auto load = [&](int group) {
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int blk = group * SCORE_GROUP + 16 * warp + g + 8 * e;
+      const int64_t at = blk < nb ? bounds_index(p.c, b, kh, blk) : -1;
+      there[e] = at >= 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        lo[e][j] = hi[e][j] = make_uint4(0, 0, 0, 0);
+        if (at >= 0) {
+          lo[e][j] = *(const uint4*)(p.bounds + at * 2 * AD + 32 * j + 8 * tg);
+          hi[e][j] = *(const uint4*)(p.bounds + at * 2 * AD + AD + 32 * j + 8 * tg);
+        }
+      }
+    }
+  };
+  load(blockIdx.x);
+  for (int i = warp; i < T * GQA; i += SCORE_WARPS) {
+    const int t = i / GQA, h = i % GQA;
+    const float* src = p.qn + (((size_t)b * T + t) * nqh + kh * GQA + h) * AD + 8 * lane;
+    float x[8], amax = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = src[k], amax = fmaxf(amax, fabsf(x[k]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const int e = (int)(__float_as_uint(amax) >> 23) - 127;  // amax < 2^(e + 1)
+    const int up = min(9 - e, 100);
+    const float scale = __uint_as_float((uint32_t)(127 + up) << 23);
+    if (lane == 0) unit[t][h] = __uint_as_float((uint32_t)(127 - up) << 23);
+    uint32_t w[Q_PARTS][4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float a = x[2 * k] * scale, c = x[2 * k + 1] * scale;
+      const __half2 h2 = __floats2half2_rn(a, c);
+      const float2 f = __half22float2(h2);
+      const __half2 l2 = __floats2half2_rn(a - f.x, c - f.y);
+      const uint32_t pos = (a < 0.f ? 0u : 0xFFFFu) | (c < 0.f ? 0u : 0xFFFF0000u);  // by the sign of q itself
+      w[QP_HI][k] = h2_as_u32(h2) & pos;
+      w[QM_HI][k] = h2_as_u32(h2) & ~pos;
+      w[QP_LO][k] = h2_as_u32(l2) & pos;
+      w[QM_LO][k] = h2_as_u32(l2) & ~pos;
+      w[QABS][k] = h2_as_u32(__hadd2(__habs2(h2), __half2half2(__ushort_as_half((unsigned short)0x2400))));  // + 2^-6
+    }
+#pragma unroll
+    for (int k = 0; k < Q_PARTS; k++)
+      *(uint4*)&sq[t * Q_TOKEN + (k * 8 + h) * Q_STRIDE + 16 * lane] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int group = blockIdx.x; group < ngroups; group += gridDim.x) {
+    if (group != (int)blockIdx.x) load(group);
+#pragma unroll 1
+    for (int t = 0; t < T; t++) {
+      const uint8_t* qt = sq + t * Q_TOKEN + g * Q_STRIDE + 16 * tg;
+      float sp[4] = {}, sm[4] = {}, sl[4] = {}, sa[4] = {};
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        uint4 q[Q_PARTS];
+#pragma unroll
+        for (int k = 0; k < Q_PARTS; k++) q[k] = *(const uint4*)(qt + k * 8 * Q_STRIDE + 64 * j);
+        const uint4 l0 = lo[0][j], l1 = lo[1][j], h0 = hi[0][j], h1 = hi[1][j];
+        mma16816(sp, h0.x, h1.x, h0.y, h1.y, q[QP_HI].x, q[QP_HI].y);
+        mma16816(sm, l0.x, l1.x, l0.y, l1.y, q[QM_HI].x, q[QM_HI].y);
+        mma16816(sl, h0.x, h1.x, h0.y, h1.y, q[QP_LO].x, q[QP_LO].y);
+        mma16816(sp, h0.z, h1.z, h0.w, h1.w, q[QP_HI].z, q[QP_HI].w);
+        mma16816(sm, l0.z, l1.z, l0.w, l1.w, q[QM_HI].z, q[QM_HI].w);
+        mma16816(sl, l0.x, l1.x, l0.y, l1.y, q[QM_LO].x, q[QM_LO].y);
+        mma16816(sl, h0.z, h1.z, h0.w, h1.w, q[QP_LO].z, q[QP_LO].w);
+        mma16816(sl, l0.z, l1.z, l0.w, l1.w, q[QM_LO].z, q[QM_LO].w);
+        const auto widest = [](uint32_t x, uint32_t y) { return h2_as_u32(__hmax2_nan(__habs2(u32_as_h2(x)), __habs2(u32_as_h2(y)))); };
+        mma16816(sa, widest(l0.x, h0.x), widest(l1.x, h1.x), widest(l0.y, h0.y), widest(l1.y, h1.y), q[QABS].x, q[QABS].y);
+        mma16816(sa, widest(l0.z, h0.z), widest(l1.z, h1.z), widest(l0.w, h0.w), widest(l1.w, h1.w), q[QABS].z, q[QABS].w);
+      }
+      // rows g and g + 8, heads 2 tg and 2 tg + 1
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        float best = -INFINITY, err = 0.f;
+        bool odd = false;  // something is no finite number
+        if (tg < 3) {
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const float u = unit[t][2 * tg + i], v = (sp[2 * e + i] + sm[2 * e + i] + sl[2 * e + i]) * u, a = sa[2 * e + i] * u * 6.2e-5f;
+            odd |= !(fabsf(v) <= 3e38f) || !(a <= 3e38f);
+            best = fmaxf(best, v);
+            err = fmaxf(err, a);
+          }
+        }
+        if (odd) err = INFINITY;
+#pragma unroll
+        for (int o = 1; o <= 2; o <<= 1) {
+          best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+          err = fmaxf(err, __shfl_xor_sync(0xffffffffu, err, o));
+        }
+        const int blk = group * SCORE_GROUP + 16 * warp + g + 8 * e;
+        if (tg == 0 && blk < nb)
+          p.score[(((size_t)b * T + t) * p.c.nkvh + kh) * p.max_blocks + blk] = there[e] ? make_float2(best, err) : make_float2(-3e38f, 0.f);
+      }
+    }
+  }
+}
+
+constexpr int SEL_THREADS = 512, SEL_WARPS = SEL_THREADS / 32, SEL_BITS = 11, SEL_BINS = 1 << SEL_BITS;
+static_assert(SEL_MAX_BLOCKS <= 32 * SEL_THREADS, "a word of 32 blocks per thread");
+
+struct SelShared {
+  unsigned int hist[SEL_BINS];
+  unsigned long long sums[SEL_WARPS];
+  uint64_t key_red[2][SEL_WARPS];
+  float red[SEL_WARPS];
+  int bin, need, inside, n_in, n_open;
+  uint32_t in[SEL_MAX_BLOCKS / 32], edge[SEL_MAX_BLOCKS / 32];  // a bit per block: is chosen; is chosen while there is room
+};
+
+// Exclusive sum over the block of x (two counts, 32 bits each).
+__device__ __forceinline__ unsigned long long block_scan(unsigned long long x, unsigned long long* sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long v = x;
 #pragma unroll
@@ -191,133 +334,254 @@ __device__ __forceinline__ unsigned long long block_scan(unsigned long long x, u
   }
   if (lane == 31) sums[warp] = v;
   __syncthreads();
-  unsigned long long before = 0, all = 0;
-  for (int w = 0; w < SEL_THREADS / 32; w++) {
-    if (w < warp) before += sums[w];
-    all += sums[w];
-  }
+  unsigned long long before = 0;
+#pragma unroll
+  for (int w = 0; w < SEL_WARPS; w++) before += w < warp ? sums[w] : 0;
   __syncthreads();
-  *total = all;
   return before + v - x;
 }
 
+// Keys whose order is that of the numbers: larger number, larger key; -0 as 0; NaN (64 bits) above all.
+__device__ __forceinline__ uint32_t order_key(float s) {
+  const uint32_t bits = __float_as_uint(s + 0.f);
+  return bits >> 31 ? ~bits : bits | 0x80000000u;
+}
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
+__device__ __forceinline__ uint64_t order_key(double s) {
+  if (s != s) return ~0ull;
+  const uint64_t bits = (uint64_t)__double_as_longlong(s + 0.0);
+  return bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
+}
+
+// Where the want-th largest (1 <= want <= n) of key(0) .. key(n - 1) lies, all 512 threads: eleven bits at a time from the
+// highest bit in which keys differ, until at most `few` keys share its leading bits. Returns those bits; *mask_out which they
+// are, *need_out how many of the keys that share them belong to the want largest. hist is zero on entry and on return.
+template <typename K, typename F>
+__device__ K nth_largest(F key, int n, int want, int few, SelShared& sh, K* mask_out, int* need_out) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int BITS = 8 * sizeof(K), PER = SEL_BINS / SEL_THREADS;
+  K mn = ~(K)0, mx = 0;
+  for (int i = tid; i < n; i += SEL_THREADS) mn = min(mn, key(i)), mx = max(mx, key(i));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    mn = min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  if (lane == 0) sh.key_red[0][warp] = mn, sh.key_red[1][warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < SEL_WARPS; w++) mn = min(mn, (K)sh.key_red[0][w]), mx = max(mx, (K)sh.key_red[1][w]);
+  const int top = 64 - __clzll((long long)(uint64_t)(K)(mn ^ mx));  // keys agree above the lowest `top` bits
+  int need = want, shift = max(0, top - SEL_BITS), inside = n;
+  K mask = top >= BITS ? (K)0 : (K)(~(K)0 << top), prefix = mn & mask;
+  while (mask != ~(K)0 && inside > few) {
+    for (int i = tid; i < n; i += SEL_THREADS) {
+      const K x = key(i);
+      if ((x & mask) == prefix) atomicAdd(&sh.hist[(unsigned)(x >> shift) & (SEL_BINS - 1)], 1u);
+    }
+    __syncthreads();
+    // thread i looks at the four bins from 2047 - 4 i down
+    unsigned int h[PER], mine = 0;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      mine += h[j] = sh.hist[SEL_BINS - 1 - (PER * tid + j)];
+      sh.hist[SEL_BINS - 1 - (PER * tid + j)] = 0;
+    }
+    int above = (int)block_scan(mine, sh.sums);
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+      if (above < need && above + (int)h[j] >= need) {
+        sh.bin = SEL_BINS - 1 - (PER * tid + j);
+        sh.need = need - above;
+        sh.inside = (int)h[j];
+      }
+      above += (int)h[j];
+    }
+    __syncthreads();
+    need = sh.need;
+    inside = sh.inside;
+    prefix |= (K)sh.bin << shift;
+    mask |= (K)(SEL_BINS - 1) << shift;
+    shift = max(0, shift - SEL_BITS);
+    __syncthreads();
+  }
+  *mask_out = mask;
+  *need_out = need;
+  return prefix;
+}
+
+// The choice of one (token, KV head, sequence). With s the score to 15 bits, e its error, E the largest e and [t0, t1] an interval
+// that holds the want-th largest s: want blocks or more have a score of at least t0 - E, so a block of s + e < t0 - E is
+// out; the scores of the blocks with s <= t1 are at most t1 + E, and fewer than want have a larger s, so a block of s - e > t1 + E
+// is in. The blocks between are scored again in 64 bits, a warp each, and the best of them fill up the list; of equal ones the
+// lower. Where something is not finite, or everything alike, these are all blocks. Bound by the latency of a dozen barriers.
 __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectParams p) {
-  extern __shared__ unsigned long long keys[];
-  __shared__ double q[GQA][AD];
-  __shared__ unsigned long long sums[SEL_THREADS / 32];
-  __shared__ unsigned int hist[256];
-  __shared__ unsigned long long s_prefix;
-  __shared__ int s_need, s_done;
+  extern __shared__ uint64_t dyn[];  // [max_blocks] (score, error), then the 64-bit keys of the open blocks; then their numbers
+  __shared__ SelShared sh;
   pdl_trigger();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int kh = blockIdx.x, t = blockIdx.y, b = blockIdx.z, nqh = p.c.nkvh * GQA;
-  int* out = p.sel + (((size_t)b * p.c.T + t) * p.c.nkvh + kh) * p.k;
+  const size_t tok = (size_t)b * p.c.T + t, row = tok * p.c.nkvh + kh;
+  int* out = p.sel + row * p.k;
+  for (int i = tid; i < SEL_BINS; i += SEL_THREADS) sh.hist[i] = 0;
+  if (tid == 0) sh.n_open = 0, sh.n_in = 0;
   pdl_wait();
-  const int last_pos = min(first_pos(p.c, b) + t, p.c.n_ctx - 1);
-  const int nb = last_pos < 0 ? 0 : last_pos / BLK + 1;  // blocks up to the token's own
-  const int sink = min(p.n_sink, nb), recent = min(p.n_recent, nb - sink), lo = sink, hi = nb - recent;
-  const int want = p.k - sink - recent;  // of the blocks [lo, hi)
+  const int nb = blocks_of(p.c, b, t);
   if (nb <= p.k) {
     for (int i = tid; i < p.k; i += SEL_THREADS) out[i] = i < nb ? i : -1;
     return;
   }
-  const float* qn = p.qn + (((size_t)b * p.c.T + t) * nqh + kh * GQA) * AD;
-  for (int i = tid; i < GQA * AD; i += SEL_THREADS) (&q[0][0])[i] = (double)qn[i];
+  const int lo = p.n_sink, hi = nb - p.n_recent, n = hi - lo;  // k < nb: both ends are whole and apart
+  const int want = p.k - p.n_sink - p.n_recent;                // of the blocks [lo, hi); fewer than n
+  const int words = (nb + 31) / 32;
+  float2* score = (float2*)dyn;
+  uint16_t* open = (uint16_t*)(dyn + p.max_blocks);
+  float E = 0.f, above = INFINITY, below = INFINITY;  // want = 0: nothing between the ends
+  if (want > 0) {
+    const float2* src = p.score + row * p.max_blocks + lo;
+    for (int i = tid; i < n; i += SEL_THREADS) {
+      const float2 v = src[i];
+      score[i] = v;
+      E = fmaxf(E, v.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) E = fmaxf(E, __shfl_xor_sync(0xffffffffu, E, o));
+    if (lane == 0) sh.red[warp] = E;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SEL_WARPS; w++) E = fmaxf(E, sh.red[w]);
+    if (E <= 3e38f) {
+      uint32_t mask;
+      int ignored;
+      const uint32_t lead = nth_largest<uint32_t>([&](int i) { return order_key(score[i].x); }, n, want, 16, sh, &mask, &ignored);
+      above = key_value(lead | ~mask) + E;
+      below = key_value(lead) - E;
+    } else {
+      below = -INFINITY;  // all are open (no s - e is above infinity)
+    }
+  }
+  for (int w = warp; w < words; w += SEL_WARPS) {
+    const int blk = 32 * w + lane;
+    bool in = blk < lo || (blk >= hi && blk < nb), maybe = false;
+    if (blk >= lo && blk < hi && want > 0) {
+      const float2 v = score[blk - lo];
+      in = v.x - v.y > above;
+      maybe = !in && !(v.x + v.y < below);
+    }
+    const uint32_t wi = __ballot_sync(0xffffffffu, in), wo = __ballot_sync(0xffffffffu, maybe);
+    int at = 0;
+    if (lane == 0) {
+      sh.in[w] = wi;
+      sh.edge[w] = 0;
+      if (wo) at = atomicAdd(&sh.n_open, __popc(wo));
+      if (wi) atomicAdd(&sh.n_in, __popc(wi));
+    }
+    at = __shfl_sync(0xffffffffu, at, 0);
+    if (maybe) open[at + __popc(wo & ((1u << lane) - 1))] = (uint16_t)blk;
+  }
   __syncthreads();
-  for (int blk = lo + warp; blk < hi; blk += SEL_THREADS / 32) {
-    const int64_t at = bounds_index(p.c, b, kh, blk);
-    double s[GQA] = {};
-    if (at >= 0) {
-      const uint4 l4 = *(const uint4*)(p.bounds + at * 2 * AD + 8 * lane), h4 = *(const uint4*)(p.bounds + at * 2 * AD + AD + 8 * lane);
-      const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
+  const int n_open = sh.n_open, room = p.k - sh.n_in;  // 0 <= room <= n_open, by the above
+  int need = 0;
+  if (room == n_open) {
+    for (int c = tid; c < n_open; c += SEL_THREADS) atomicOr(&sh.in[open[c] >> 5], 1u << (open[c] & 31));
+    __syncthreads();
+  } else {
+    uint64_t* key = dyn;  // the scores to 15 bits are no longer used
+    float q[GQA][8];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float2 lf = __half22float2(u32_as_h2(lw[i >> 1])), hf = __half22float2(u32_as_h2(hw[i >> 1]));
-        const double l = i & 1 ? lf.y : lf.x, h = i & 1 ? hf.y : hf.x;
+    for (int g = 0; g < GQA; g++)
 #pragma unroll
-        for (int g = 0; g < GQA; g++) {
-          const double x = q[g][8 * lane + i];
-          s[g] = fma(x, x < 0.0 ? l : h, s[g]);
+      for (int i = 0; i < 8; i++) q[g][i] = p.qn[(tok * nqh + kh * GQA + g) * AD + 8 * lane + i];
+    for (int c = warp; c < n_open; c += SEL_WARPS) {
+      const int64_t idx = bounds_index(p.c, b, kh, open[c]);
+      double s[GQA] = {};
+      if (idx >= 0) {
+        const uint4 l4 = *(const uint4*)(p.bounds + idx * 2 * AD + 8 * lane), h4 = *(const uint4*)(p.bounds + idx * 2 * AD + AD + 8 * lane);
+        const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float2 lf = __half22float2(u32_as_h2(lw[i >> 1])), hf = __half22float2(u32_as_h2(hw[i >> 1]));
+#pragma unroll
+          for (int g = 0; g < GQA; g++) {
+            const double x = q[g][i];
+            s[g] = fma(x, (double)(q[g][i] < 0.f ? (i & 1 ? lf.y : lf.x) : (i & 1 ? hf.y : hf.x)), s[g]);
+          }
         }
       }
-    }
-    double best = -INFINITY;
-    bool nan = false;
+      double best = -INFINITY;
+      bool nan = false;
 #pragma unroll
-    for (int g = 0; g < GQA; g++) {
+      for (int g = 0; g < GQA; g++) {
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
-      nan |= s[g] != s[g];
-      best = fmax(best, s[g]);
-    }
-    if (lane == 0) keys[blk - lo] = at < 0 ? 0ull : nan ? ~0ull : score_key(best);
-  }
-  __syncthreads();
-  // The want-th largest key, eight bits at a time from the top; done early when a bin holds just what is still wanted.
-  const int n = hi - lo;
-  if (tid == 0) s_prefix = 0, s_need = want, s_done = 0;
-  int shift = 56;
-  unsigned long long mask = 0;
-  __syncthreads();
-  if (want > 0) {
-    for (; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += SEL_THREADS) hist[i] = 0;
-      __syncthreads();
-      const unsigned long long prefix = s_prefix;
-      for (int i = tid; i < n; i += SEL_THREADS)
-        if ((keys[i] & mask) == prefix) atomicAdd(&hist[(unsigned)(keys[i] >> shift) & 255u], 1u);
-      __syncthreads();
-      if (tid == 0) {
-        int need = s_need, d = 255;
-        while ((int)hist[d] < need) need -= (int)hist[d--];
-        s_need = need;
-        s_prefix = prefix | ((unsigned long long)d << shift);
-        s_done = (int)hist[d] == need;
+        for (int o = 16; o > 0; o >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], o);
+        nan |= s[g] != s[g];
+        best = fmax(best, s[g]);
       }
-      __syncthreads();
-      mask |= 255ull << shift;
-      if (s_done) break;
+      if (lane == 0) key[c] = idx < 0 ? 0ull : nan ? ~0ull : order_key(best);
     }
+    __syncthreads();
+    if (n_open <= SEL_THREADS) {  // few: each counts those before it
+      if (tid < n_open) {
+        const uint64_t k = key[tid];
+        const int blk = open[tid];
+        int rank = 0;
+        for (int c = 0; c < n_open; c++) rank += key[c] > k || (key[c] == k && open[c] < blk);
+        if (rank < room) atomicOr(&sh.in[blk >> 5], 1u << (blk & 31));
+      }
+    } else {
+      uint64_t mask;
+      const uint64_t border = nth_largest<uint64_t>([&](int i) { return key[i]; }, n_open, room, 0, sh, &mask, &need);
+      for (int c = tid; c < n_open; c += SEL_THREADS)
+        if (key[c] >= border) atomicOr(key[c] > border ? &sh.in[open[c] >> 5] : &sh.edge[open[c] >> 5], 1u << (open[c] & 31));
+    }
+    __syncthreads();
   }
-  // Blocks above the prefix are in; of those that share it all (done early) or the first s_need.
-  const unsigned long long prefix = s_prefix;
-  const int need = want > 0 ? s_need : 0;
-  const int per = (nb + SEL_THREADS - 1) / SEL_THREADS, b0 = min(nb, tid * per), b1 = min(nb, b0 + per);
-  auto rank_of = [&](int blk) {  // 2: in, 1: shares the prefix, 0: out
-    if (blk < lo || blk >= hi) return 2;
-    if (want <= 0) return 0;
-    const unsigned long long k = keys[blk - lo] & mask;
-    return k > prefix ? 2 : k == prefix ? 1 : 0;
-  };
-  unsigned long long mine = 0, total;
-  for (int blk = b0; blk < b1; blk++) {
-    const int r = rank_of(blk);
-    mine += r == 2 ? 1ull << 32 : r == 1 ? 1ull : 0ull;
-  }
-  const unsigned long long before = block_scan(mine, sums, &total);
-  int above = (int)(before >> 32), equal = (int)(before & 0xffffffffu);
-  for (int blk = b0; blk < b1; blk++) {
-    const int r = rank_of(blk);
-    if (r == 2 || (r == 1 && equal < need)) out[above + min(equal, need)] = blk;
-    above += r == 2;
-    equal += r == 1;
+  // The list in order: what is in, and the first `need` on the edge.
+  uint32_t in = tid < words ? sh.in[tid] : 0u, edge = tid < words ? sh.edge[tid] : 0u;
+  const unsigned long long before = block_scan((unsigned long long)__popc(in) << 32 | (unsigned)__popc(edge), sh.sums);
+  int on = (int)(before & 0xffffffffu), at = (int)(before >> 32) + min(on, need);
+  for (uint32_t m = in | edge; m; m &= m - 1) {
+    const int bit = __ffs((int)m) - 1;
+    if ((edge >> bit) & 1 && on++ >= need) continue;
+    out[at++] = 32 * tid + bit;
   }
 }
 
-int launch_select(const SelectParams& p, int max_len, cudaStream_t s) {
+int launch_select(DeviceCtx* ctx, SelectParams& p, int max_len, const char* who, cudaStream_t s) {
   static bool attr[64] = {};
   static std::mutex attr_mu;
-  int dev;
-  Q27B_CK(cudaGetDevice(&dev));
+  auto smem_of = [](int blocks) { return (size_t)blocks * 10; };  // a 64-bit key and a number of every block
   {
     std::lock_guard<std::mutex> lock(attr_mu);
-    if (!attr[dev]) {
-      Q27B_CK(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_MAX_BLOCKS * 8));
-      attr[dev] = true;
+    if (!attr[ctx->dev]) {
+      Q27B_CK(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(SEL_MAX_BLOCKS)));
+      Q27B_CK(cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Q27B_MAX_T * Q_TOKEN));
+      attr[ctx->dev] = true;
     }
   }
-  const size_t smem = (size_t)((max_len + BLK - 1) / BLK) * 8;
-  Q27B_CK(launch_step(select_kernel, dim3(p.c.nkvh, p.c.T, p.c.B), dim3(SEL_THREADS), smem, s, p));
+  p.max_blocks = (max_len + BLK - 1) / BLK;
+  const bool scored = p.max_blocks > p.k;
+  if (scored) {
+    const size_t floats = (size_t)p.c.B * p.c.T * p.c.nkvh * p.max_blocks * 2;
+    float* scratch;
+    if (p.c.page_table) {
+      if (int rc = paged_ws(ctx, floats, &scratch)) return rc;
+    } else {
+      size_t cap;
+      if (int rc = prefill_ws(ctx, &scratch, &cap)) return rc;
+      if (cap < floats)
+        return fail(Q27B_UNSUPPORTED, std::string(who) + ": the prefill workspace (" + std::to_string(cap * sizeof(float)) +
+                                          " bytes) is too small for the scores of this call (" +
+                                          std::to_string(floats * sizeof(float)) + " bytes)");
+    }
+    p.score = (float2*)scratch;
+    // Two CTAs fit an SM; twice as many as that, where the blocks suffice, even out sequences of different length. A CTA
+    // goes through several groups of 64 blocks with the queries staged once.
+    const int64_t pairs = (int64_t)p.c.nkvh * p.c.B, groups = (p.max_blocks + SCORE_GROUP - 1) / SCORE_GROUP;
+    const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(groups, (4 * (int64_t)ctx->n_sm + pairs - 1) / pairs));
+    Q27B_CK(launch_step(score_kernel, dim3((unsigned)ctas, p.c.nkvh, p.c.B), dim3(32 * SCORE_WARPS), p.c.T * Q_TOKEN, s, p));
+  }
+  Q27B_CK(launch_step(select_kernel, dim3(p.c.nkvh, p.c.T, p.c.B), dim3(SEL_THREADS), scored ? smem_of(p.max_blocks) : 0, s, p));
   return Q27B_OK;
 }
 
@@ -391,7 +655,7 @@ int q27b_select_blocks(const float* qn, const void* bounds, int* sel, const int*
   SelectParams p = {};
   p.c = contiguous_ref(ctx, pos0, T, nkvh, n_ctx, 1);
   p.qn = qn; p.bounds = (const __half*)bounds; p.sel = sel; p.k = k; p.n_sink = n_sink; p.n_recent = n_recent;
-  return launch_select(p, n_ctx, (cudaStream_t)stream);
+  return launch_select(ctx, p, n_ctx, "select_blocks", (cudaStream_t)stream);
 }
 
 int q27b_select_blocks_paged(const float* qn, const void* bounds, int* sel, const int* page_table, const int* seq_len, int B,
@@ -407,7 +671,7 @@ int q27b_select_blocks_paged(const float* qn, const void* bounds, int* sel, cons
   p.c = paged_ref(ctx, page_table, seq_len, B, T, nkvh, n_pages, max_pages);
   p.c.n_ctx = max_seq_len;  // a longer sequence than the caller said is cut there: the scores have room for no more
   p.qn = qn; p.bounds = (const __half*)bounds; p.sel = sel; p.k = k; p.n_sink = n_sink; p.n_recent = n_recent;
-  return launch_select(p, max_seq_len, (cudaStream_t)stream);
+  return launch_select(ctx, p, max_seq_len, "select_blocks_paged", (cudaStream_t)stream);
 }
 
 }  // extern "C"
