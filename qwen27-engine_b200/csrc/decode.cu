@@ -30,6 +30,7 @@
 #include "combine.h"
 #include "common.cuh"
 #include "decode_params.h"
+#include "sel_list.cuh"
 
 #include <algorithm>
 #include <atomic>
@@ -82,6 +83,9 @@ constexpr int OFF_TOK = OFF_FLAG + 16;                      // [groups][2 buffer
 constexpr int SMEM_USED = OFF_TOK + 32;
 constexpr float TAU = 8.0f;                                 // a score may exceed the reference max by this much
 constexpr int SMEM_BYTES = SMEM_USED + 1024;               // slack for the 1024-byte alignment of the ring
+constexpr int OFF_LIST = (SMEM_USED + 15) / 16 * 16;        // lists of blocks: [SEL_CHUNK] tiles and their number
+constexpr int SEL_SMEM_BYTES = OFF_LIST + SEL_CHUNK * 4 + 16 + 1024;
+static_assert(SEL_SMEM_BYTES <= 232448, "shared memory budget of one CTA");
 constexpr int O_STRIDE = AD + 4;                            // floats per row of the end-of-kernel O exchange
 static_assert((NGROUP - 1) * MAXR * O_STRIDE * 4 <= RING_BYTES, "O exchange must fit in the ring");
 static_assert(NGROUP == 2, "the register budget (Q fragments in registers) is sized for two groups");
@@ -132,8 +136,8 @@ __device__ __forceinline__ int ks_dim0(int ks, int tg) {
 }
 
 // NT = 8-row groups of query rows (ceil(6 T / 8)). PAGED: batched decode over 256-position pages
-// (q8_0 only). Q8: q8_0 cache (else f16).
-template <int NT, bool PAGED, bool Q8>
+// (q8_0 only). Q8: q8_0 cache (else f16). SEL: every token (grid z) attends its own list of blocks, a chunk is a part of it.
+template <int NT, bool PAGED, bool Q8, bool SEL = false>
 __global__ void __launch_bounds__(N_THREADS, 1)
 decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_ks,
               const __grid_constant__ CUtensorMap tm_vv, const __grid_constant__ CUtensorMap tm_vs,
@@ -163,8 +167,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
   pdl_trigger();  // after the wait: when the merge kernel's CTAs start, everything before this kernel has completed
   const int ch = blockIdx.x, kh = blockIdx.y;
   const int T = p.T, R = GQA * T;
-  const int seq = PAGED ? blockIdx.z : 0;
-  const int pos0 = PAGED ? p.seq_len[seq] - T : *p.pos0;
+  const int seq = PAGED || SEL ? blockIdx.z : 0;
+  const int pos0 = SEL ? sel_pos(p, PAGED, seq) : PAGED ? p.seq_len[seq] - T : *p.pos0;
   const float* qn = p.qn + (size_t)seq * T * p.nqh * AD;
   const int g = lane >> 2, tg = lane & 3;
 
@@ -182,16 +186,23 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
   const int c0 = min(n, ch * chunk), c1 = min(n, c0 + chunk);
   float* out = p.part + (((size_t)seq * p.nkvh + kh) * p.nch + ch) * MAXR * PROW;
 
-  if (c0 >= c1) {
+  if (!SEL && c0 >= c1) {
     // Empty chunk: what the merge reads of it is the neutral partial (src/attn.cu:117-120). It reads only the
     // partials that hold something (filled_chunks; with pages the chunks that a sequence has).
     if (!PAGED && ch < filled_chunks(n, p.nch))
       for (int i = tid; i < R * PROW; i += N_THREADS) out[i] = (i % PROW == 0) ? M_INIT : 0.f;
     return;
   }
-  const int ntiles = (c1 - c0 + TILE - 1) / TILE;
+  int ntiles = (c1 - c0 + TILE - 1) / TILE;
+  int* const list = (int*)(sgen + OFF_LIST);
+  if (SEL && warp == 0) {
+    const int c = collect_blocks(p, PAGED, seq, kh, ch * p.chunk_len, min(p.sel_k, (ch + 1) * p.chunk_len), n, list);
+    if (lane == 0) list[SEL_CHUNK] = c;
+  }
 
   __syncthreads();
+  if (SEL) ntiles = list[SEL_CHUNK];  // may be 0: the partial is then the neutral one
+  const int seen_end = SEL ? n : c1;  // rows from here on are not seen
 
   // TMA of tile `it` into stage it % NSTAGE (one thread).
   const int row0 = kh * p.n_ctx + c0;
@@ -199,7 +210,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
     uint8_t* st = sgen + (size_t)(it % NSTAGE) * G::STAGE_BYTES;
     uint64_t* bar = &full[it % NFULL];
     mbar_expect_tx(bar, G::STAGE_BYTES);
-    int row = row0 + it * TILE;
+    int row = SEL ? kh * p.n_ctx + list[it] * TILE : row0 + it * TILE;
     if (PAGED) {  // a tile never straddles a page (64 | 256)
       const int pp = c0 + it * TILE;
       int pg = p.page_table[(size_t)seq * p.max_pages + pp / Q27B_PAGE];
@@ -255,9 +266,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       const int r = 8 * nt + 2 * tg + e;
-      lim[nt][e] = min(c1, pos0 + min(r / GQA, T - 1) + 1 - p.base_pos);
+      lim[nt][e] = min(seen_end, pos0 + min(r / GQA, T - 1) + 1 - p.base_pos);
     }
-  const int lim_min = min(c1, pos0 + 1 - p.base_pos);
+  const int lim_min = min(seen_end, pos0 + 1 - p.base_pos);
 
   float o[4][NT][4];
 #pragma unroll
@@ -292,7 +303,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
   for (int it = grp; it < ntiles; it += NGROUP, jt++) {
     mbar_wait(&full[it % NFULL], (it / NFULL) & 1, abort_flag, p.status);
     const uint32_t st = sbase + (it % NSTAGE) * G::STAGE_BYTES;
-    const int tile_p0 = c0 + it * TILE;
+    const int tile_p0 = SEL ? list[it] * TILE : c0 + it * TILE;
     const bool edge = tile_p0 + TILE > lim_min;  // some row of the tile is masked for some query row
 
     // ---- S^T = K Q^T for tile rows ra, rb
@@ -439,10 +450,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
           uint32_t sa = ldsu16(st + sA + ks * 256), sb = ldsu16(st + sA + ks * 256 + 128);
           uint32_t scc = ldsu16(st + sA + ks * 256 + 16), sd = ldsu16(st + sA + ks * 256 + 144);
           if (edge) {  // rows past the end of the sequence may hold anything: make them exact zeros
-            if (tile_p0 + pa >= c1) sa = 0;
-            if (tile_p0 + pb >= c1) sb = 0;
-            if (tile_p0 + pc >= c1) scc = 0;
-            if (tile_p0 + pd >= c1) sd = 0;
+            if (tile_p0 + pa >= seen_end) sa = 0;
+            if (tile_p0 + pb >= seen_end) sb = 0;
+            if (tile_p0 + pc >= seen_end) scc = 0;
+            if (tile_p0 + pd >= seen_end) sd = 0;
           }
           const __half2 sab = u32_as_h2(prmt(sa, sb, 0x5410)), scd = u32_as_h2(prmt(scc, sd, 0x5410));
           const uint32_t xaw[2] = {xa.x, xa.y}, xbw[2] = {xb.x, xb.y}, xcw[2] = {xc.x, xc.y}, xdw[2] = {xd.x, xd.y};
@@ -471,10 +482,10 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
           uint4 xa = lds128(vbase + swz128(pa, g)), xb = lds128(vbase + swz128(pb, g));
           uint4 xc = lds128(vbase + swz128(pc, g)), xd = lds128(vbase + swz128(pd, g));
           if (edge) {  // rows past the end of the sequence may hold anything: make them exact zeros
-            if (tile_p0 + pa >= c1) xa = make_uint4(0, 0, 0, 0);
-            if (tile_p0 + pb >= c1) xb = make_uint4(0, 0, 0, 0);
-            if (tile_p0 + pc >= c1) xc = make_uint4(0, 0, 0, 0);
-            if (tile_p0 + pd >= c1) xd = make_uint4(0, 0, 0, 0);
+            if (tile_p0 + pa >= seen_end) xa = make_uint4(0, 0, 0, 0);
+            if (tile_p0 + pb >= seen_end) xb = make_uint4(0, 0, 0, 0);
+            if (tile_p0 + pc >= seen_end) xc = make_uint4(0, 0, 0, 0);
+            if (tile_p0 + pd >= seen_end) xd = make_uint4(0, 0, 0, 0);
           }
           const uint32_t xaw[4] = {xa.x, xa.y, xa.z, xa.w}, xbw[4] = {xb.x, xb.y, xb.z, xb.w};
           const uint32_t xcw[4] = {xc.x, xc.y, xc.z, xc.w}, xdw[4] = {xd.x, xd.y, xd.z, xd.w};
@@ -545,7 +556,8 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
         f[0] = ex2((m[nt][e] - M) * LOG2E);
 #pragma unroll
         for (int k = 1; k < NGROUP; k++) f[k] = ex2((mg[k] - M) * LOG2E);
-        float* po = out + (size_t)r * PROW;
+        const size_t at = ((size_t)seq * p.nqh + kh * GQA + r) * p.nch + ch;  // SEL: [row][chunk]
+        float* po = SEL ? p.part_o + at * AD - 2 : out + (size_t)r * PROW;
 #pragma unroll
         for (int mt = 0; mt < 4; mt++) {
           const int d = 64 * wq + 8 * g + 2 * mt;
@@ -566,8 +578,12 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
             for (int w = 0; w < 4; w++) lk += ldsf(sbase + OFF_L + ((k * 4 + w) * MAXR + r) * 4);
             lsum += lk * f[k];
           }
-          po[0] = M;
-          po[1] = lsum;
+          if (SEL) {
+            p.part_ml[at] = make_float2(M, lsum);
+          } else {
+            po[0] = M;
+            po[1] = lsum;
+          }
         }
       }
   }
@@ -717,6 +733,22 @@ int noalloc_setup(int dev) {
 }
 
 }  // namespace
+
+int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const DecodeParams& p, int nseq, cudaStream_t s) {
+  static bool attr[64] = {};
+  int dev;
+  Q27B_CK(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(g_setup_mu);
+    if (!attr[dev]) {
+      Q27B_CK(cudaFuncSetAttribute(decode_kernel<1, false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_SMEM_BYTES));
+      attr[dev] = true;
+    }
+  }
+  // (the maps of scales are not read)
+  Q27B_CK(launch_step(decode_kernel<1, false, false, true>, dim3(p.nch, p.nkvh, nseq), dim3(N_THREADS), SEL_SMEM_BYTES, s, *kv, *kv, *vv, *vv, p));
+  return Q27B_OK;
+}
 
 // Reads (and clears) the status word that the no-allocation entry point's kernels report into; 0 when
 // that entry point has not run on this device. Copies from the library's own device array: allocates nothing.

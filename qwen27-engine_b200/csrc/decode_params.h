@@ -21,6 +21,12 @@ struct DecodeParams {
   // Tile pool of the warp-specialised kernel (one sequence only): [KV head] tiles drawn so far,
   // [32] CTAs that are done; all zero between launches. Null: every CTA keeps to its own share.
   int* sched;
+  // Lists of blocks (decode over selected blocks, T = 1, one "sequence" per (sequence, token)): [B][sel_T][nkvh][sel_k]
+  // 64-position blocks, -1 = none, chunk_len entries to a chunk; the partials go to part_o [row][nch][256] and part_ml [row][nch].
+  const int* sel;
+  int sel_k, sel_T;
+  float* part_o;
+  float2* part_ml;
   // measurement hook (null in normal use): [CTA][8] globaltimer stamps of the warp-specialised kernel
   unsigned long long* trace;
 };
@@ -36,6 +42,9 @@ __host__ __device__ inline int filled_chunks(int n, int nch) {
   return tiles < 1 ? 1 : (tiles + share - 1) / share;
 }
 
+// Entries of a list that a CTA takes at most.
+constexpr int SEL_CHUNK = 128;
+
 // Split-K decode over a q8_0 cache on the tcgen05 path (decode_tc.cu). Same grid, same partial
 // layout and same tensor maps as the warp-MMA kernel. paged: rows through the page table.
 int launch_decode_tc(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
@@ -50,6 +59,11 @@ int launch_decode_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtenso
 // The same with the P V contraction on tcgen05 (decode_wt.cu).
 int launch_decode_wt(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                      const DecodeParams& p, bool paged, int nseq, cudaStream_t s);
+// Decode over lists of blocks: the warp-specialised kernel (q8_0, p.page_table null: contiguous; groups as above) and the
+// single-role kernel of decode.cu (f16 caches). nseq = B * sel_T.
+int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                     const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups);
+int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const DecodeParams& p, int nseq, cudaStream_t s);
 // Opts the kernels of decode_ws.cu into their shared-memory size on the current device.
 int decode_ws_setup();
 

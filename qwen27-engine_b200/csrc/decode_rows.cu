@@ -4,113 +4,15 @@
 // y = sigmoid(gate) * sum_p P_p v_p with P the softmax of kq_scale * q.k over the visible rows p, in f32; 0 where a row
 // sees nothing. Rows that are not visible are not read, whatever they hold.
 //
-// One CTA takes the six query rows of a (token, KV head) over one share of its positions: a warp per position, eight
-// dims a lane; m, l and O of each warp are merged at the end and written as a partial, and a second kernel merges the
-// partials of a row.
+// The split kernels leave the partials (m, l, O) of a row for every share of its positions; the kernel here merges them. Trees:
+// decode_tree.cu. Lists of blocks: the split-K kernels of decode_ws.cu (q8_0) and decode.cu (f16), a chunk of a list a CTA,
+// every (token, KV head) for itself.
 #include "cache_ref.h"
+#include "decode_params.h"
 #include "decode_rows.h"
 
 namespace q27b {
 namespace {
-
-constexpr int WARPS = 8;
-
-// Eight values of a stored row as f32.
-__device__ __forceinline__ void load8(const uint8_t* base, size_t scales, bool q8, size_t row, int lane, float (&x)[8]) {
-  if (q8) {
-    const uint2 v = *(const uint2*)(base + row * AD + 8 * lane);
-    const float d = __half2float(*(const __half*)(base + scales + row * 16 + (lane >> 2) * 2));
-    const int8_t* b = (const int8_t*)&v;
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = (float)b[i] * d;
-  } else {
-    const uint4 v = *(const uint4*)(base + row * 2 * AD + 16 * lane);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 f = __half22float2(u32_as_h2(w[i]));
-      x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    }
-  }
-}
-
-__global__ void __launch_bounds__(32 * WARPS) blocks_kernel(const RowsParams p) {
-  __shared__ float sm[WARPS][GQA], sl[WARPS][GQA], so[WARPS][AD];
-  pdl_trigger();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int z = blockIdx.x, kh = blockIdx.y, b = blockIdx.z / p.c.T, t = blockIdx.z % p.c.T, nqh = p.c.nkvh * GQA;
-  pdl_wait();
-  const int first = first_pos(p.c, b), n = max(0, min(first + p.c.T, p.c.n_ctx));
-  const int share = (p.k + p.nsplit - 1) / p.nsplit;
-  const int* list = p.sel + (((size_t)b * p.c.T + t) * p.c.nkvh + kh) * p.k;
-  const size_t row0 = ((size_t)b * p.c.T + t) * nqh + kh * GQA;  // the first of the six output rows
-  float q[GQA][8], o[GQA][8], m[GQA], l[GQA];
-#pragma unroll
-  for (int g = 0; g < GQA; g++) {
-    const float* src = p.qn + (row0 + g) * AD + 8 * lane;
-#pragma unroll
-    for (int i = 0; i < 8; i++) q[g][i] = src[i] * p.kq_scale, o[g][i] = 0.f;
-    m[g] = M_INIT;
-    l[g] = 0.f;
-  }
-  const size_t scales = cache_rows(p.c) * AD;
-  for (int i = z * share; i < min(p.k, (z + 1) * share); i++) {
-    const int tile = list[i];
-    if (tile == -1) continue;
-    if (tile < -1 || tile > (p.c.n_ctx - 1) / BLK) {
-      if (threadIdx.x == 0) atomicOr(p.c.status, ST_BAD_INDEX);
-      continue;
-    }
-    if (tile * BLK >= n) continue;
-    const int64_t base = cache_row(p.c, b, kh, tile * BLK);
-    if (base < 0) continue;
-    for (int r = warp; r < BLK; r += WARPS) {
-      const int pos = tile * BLK + r;
-      if (pos >= n || pos > first + t) continue;
-      float x[8], s[GQA];
-      load8((const uint8_t*)p.kcache, scales, p.c.q8, base + r, lane, x);
-#pragma unroll
-      for (int g = 0; g < GQA; g++) {
-        s[g] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) s[g] = fmaf(q[g][e], x[e], s[g]);
-#pragma unroll
-        for (int e = 16; e > 0; e >>= 1) s[g] += __shfl_xor_sync(0xffffffffu, s[g], e);
-      }
-      load8((const uint8_t*)p.vcache, scales, p.c.q8, base + r, lane, x);
-#pragma unroll
-      for (int g = 0; g < GQA; g++) {
-        const float mn = fmaxf(m[g], s[g]), f = ex2((m[g] - mn) * LOG2E), e = ex2((s[g] - mn) * LOG2E);
-        m[g] = mn;
-        l[g] = l[g] * f + e;
-#pragma unroll
-        for (int k = 0; k < 8; k++) o[g][k] = fmaf(e, x[k], o[g][k] * f);
-      }
-    }
-  }
-  if (lane == 0)
-#pragma unroll
-    for (int g = 0; g < GQA; g++) sm[warp][g] = m[g], sl[warp][g] = l[g];
-#pragma unroll
-  for (int g = 0; g < GQA; g++) {
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 8; k++) so[warp][8 * lane + k] = o[g][k];
-    __syncthreads();
-    float M = M_INIT, L = 0.f, A = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) M = fmaxf(M, sm[w][g]);
-#pragma unroll
-    for (int w = 0; w < WARPS; w++) {
-      const float f = ex2((sm[w][g] - M) * LOG2E);
-      L += sl[w][g] * f;
-      A += so[w][threadIdx.x] * f;
-    }
-    const size_t at = (row0 + g) * p.nsplit + z;
-    p.part_o[at * AD + threadIdx.x] = A;
-    if (threadIdx.x == 0) p.part_ml[at] = make_float2(M, L);
-  }
-}
 
 // Merges the partials of a row, applies the gate and writes f16, or q8_1. One CTA a row, four groups of 64 threads that
 // take every fourth partial; a row without a visible position is 0.
@@ -196,11 +98,62 @@ int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t nsplit, 
   return Q27B_OK;
 }
 
+// How lists of k blocks are cut into chunks, a CTA each: the plan of the least time in a model of the launch (us). A round of CTAs
+// costs C0 and so much a block: an SM to itself for a CTA of two tile groups 0.71 (q8_0) or 1.1 (f16), for one of one group
+// 0.97, and 1.37 where two of those share it. Measured on 14 shapes (1 to 512 lists of 16 to 1,024 blocks): 4 lists of 128
+// blocks 11.7 us in 32 chunks of two groups and 14.4 in 64 of one; 16 of 64 14.3 and 15.0; 128 of 64 54.8 in pairs of CTAs and 56.6
+// in single ones; 256 of 64 102.6 and 107.1; 256 of 16 34.1 and 39.0. The plan was within 4 % of the best of each.
+struct BlocksPlan {
+  int nch;
+  WsGroups groups;
+};
+BlocksPlan plan_blocks(int64_t lists, int k, int n_sm, bool q8) {
+  BlocksPlan best = {1, WsGroups::TWO};
+  double least = 1e300;
+  int last = 0;
+  for (int nch = (k + SEL_CHUNK - 1) / SEL_CHUNK; nch <= std::min(k, std::max(64, (k + SEL_CHUNK - 1) / SEL_CHUNK)); nch++) {
+    const int chunk = (k + nch - 1) / nch;
+    if (chunk == last) continue;  // the same chunks
+    last = chunk;
+    const int64_t ctas = lists * ((k + chunk - 1) / chunk);
+    const double merge = 4e-4 * (double)(ctas * GQA);
+    const double rounds = (double)((ctas + n_sm - 1) / n_sm);
+    const double two = rounds * (5.0 + (q8 ? 0.71 : 1.1) * chunk) + merge;
+    if (two < least) least = two, best = {(k + chunk - 1) / chunk, WsGroups::TWO};
+    if (!q8) continue;
+    const double pairs = (double)((ctas + 2 * n_sm - 1) / (2 * n_sm));
+    const double one = (ctas <= n_sm ? 5.0 + 0.97 * chunk : pairs * (5.0 + 1.37 * chunk)) + merge;
+    if (one < least) least = one, best = {(k + chunk - 1) / chunk, ctas <= n_sm ? WsGroups::SPREAD : WsGroups::PAIRED};
+  }
+  return best;
+}
+
 int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
-  const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, ctas = (int64_t)p.c.B * p.c.T * p.c.nkvh;
-  const int64_t ns = std::max<int64_t>(1, std::min<int64_t>({p.k, 64, (8 * (int64_t)ctx->n_sm + ctas - 1) / ctas}));
-  if (int rc = place_partials(ctx, p, rows, ns, who)) return rc;
-  Q27B_CK(launch_step(blocks_kernel, dim3(p.nsplit, p.c.nkvh, p.c.B * p.c.T), dim3(32 * WARPS), 0, s, p));
+  const CacheRef& c = p.c;
+  const int64_t lists = (int64_t)c.B * c.T * c.nkvh, rows = lists * GQA;
+  const BlocksPlan plan = plan_blocks(lists, p.k, ctx->n_sm, c.q8);
+  const int nch = plan.nch;
+  const WsGroups groups = plan.groups;
+  if (int rc = place_partials(ctx, p, rows, nch, who)) return rc;
+  const int chunk = (p.k + p.nsplit - 1) / p.nsplit;
+  if (chunk > SEL_CHUNK) return fail(Q27B_UNSUPPORTED, std::string(who) + ": the workspace is too small for the partials of this call");
+  p.nsplit = (p.k + chunk - 1) / chunk;
+  DecodeParams d = {};
+  d.qn = p.qn; d.pos0 = c.pos0; d.status = c.status; d.T = 1; d.nqh = c.nkvh * GQA; d.nkvh = c.nkvh; d.n_ctx = c.n_ctx;
+  d.nch = p.nsplit; d.kq_scale = p.kq_scale; d.n_local = -1; d.page_table = c.page_table; d.seq_len = c.seq_len;
+  d.max_pages = c.max_pages; d.n_pages = c.n_pages; d.chunk_len = chunk; d.sel = p.sel; d.sel_k = p.k; d.sel_T = c.T;
+  d.part_o = p.part_o; d.part_ml = p.part_ml;
+  CUtensorMap kv, ks, vv, vs;
+  const uint64_t cache = cache_rows(c);
+  if (c.q8) {
+    if (int rc = q8_tmaps(p.kcache, cache, &kv, &ks)) return rc;
+    if (int rc = q8_tmaps(p.vcache, cache, &vv, &vs)) return rc;
+    if (int rc = launch_blocks_ws(&kv, &ks, &vv, &vs, d, c.B * c.T, s, groups)) return rc;
+  } else {
+    if (int rc = cached_tmap_2d(&kv, p.kcache, cache, 2 * AD, 2 * AD, 128, BLK, true)) return rc;
+    if (int rc = cached_tmap_2d(&vv, p.vcache, cache, 2 * AD, 2 * AD, 128, BLK, true)) return rc;
+    if (int rc = launch_blocks_f16(&kv, &vv, d, c.B * c.T, s)) return rc;
+  }
   Q27B_CK(launch_step(rows_merge_kernel, dim3((unsigned)rows), dim3(256), 0, s, p));
   return Q27B_OK;
 }

@@ -44,6 +44,7 @@
 #define Q27B_INLINE_WAITS
 #include "common.cuh"
 #include "decode_params.h"
+#include "sel_list.cuh"
 
 #include <mutex>
 
@@ -89,6 +90,9 @@ struct Lay {
   static constexpr int OFF_SEQ = OFF_RTOK + 16;                      // [2 groups][8] ints: the groups' tile queues
   static constexpr int SMEM_USED = OFF_SEQ + 64;
   static constexpr int SMEM_BYTES = SMEM_USED + 1024;                // slack for the 1024-byte alignment of the ring
+  static constexpr int OFF_LIST = (SMEM_USED + 15) / 16 * 16;        // lists of blocks: [SEL_CHUNK] tiles and their number
+  static constexpr int SEL_SMEM_BYTES = OFF_LIST + SEL_CHUNK * 4 + 16 + 1024;
+  static_assert(SEL_SMEM_BYTES * (3 - NG) + (3 - NG) * 1024 <= 232448, "shared memory of one SM");
   static_assert(OFF_BAR % 8 == 0, "mbarriers are 8-byte aligned");
   static constexpr int OFF_STAGE = NG == 2 ? O_XCH_BYTES : 0;        // the chunk partial before it is written out, over the ring as well
   static_assert(OFF_STAGE + MAXR * PROW * 4 <= RING_BYTES, "O exchange and partial must fit in the ring");
@@ -150,8 +154,10 @@ __device__ __forceinline__ int slot_row(int s) { return (s & 8) | ((s & 1) << 2)
 // (a 16-byte load is 16 dims = 4 k-steps).
 __device__ __forceinline__ int ks_dim0(int ks, int tg) { return 128 * (ks >> 3) + 64 * ((ks >> 2) & 1) + 16 * tg + 4 * (ks & 3); }
 
-// NT = 8-row groups of query rows (ceil(6 T / 8)). PAGED: batched decode over 256-position pages.
-template <int NT, bool PAGED, int NG>
+// NT = 8-row groups of query rows (ceil(6 T / 8)). PAGED: batched decode over 256-position pages. SEL: every (sequence, token)
+// attends its own list of blocks; grid z is that pair, a chunk is a part of the list, and the tile numbers in the groups' queues
+// are those of the list.
+template <int NT, bool PAGED, int NG, bool SEL = false>
 __global__ void __launch_bounds__(256 * NG, 3 - NG)
 decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_ks,
                  const __grid_constant__ CUtensorMap tm_vv, const __grid_constant__ CUtensorMap tm_vs,
@@ -193,7 +199,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   pdl_trigger();  // after the wait: when the merge kernel's CTAs start, everything before this kernel has completed
   const int ch = blockIdx.x, kh = blockIdx.y;
   const int T = p.T, R = GQA * T;
-  const int seq = PAGED ? blockIdx.z : 0;
+  const int seq = PAGED || SEL ? blockIdx.z : 0;
   const float* qn = p.qn + (size_t)seq * T * p.nqh * AD;
   const int g = lane >> 2, tg = lane & 3;
 
@@ -206,7 +212,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
     qv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < R) qv[j] = *(const float4*)(qn + ((size_t)(r / GQA) * p.nqh + kh * GQA + r % GQA) * AD + 4 * c4);
   }
-  const int pos0 = PAGED ? p.seq_len[seq] - T : *p.pos0;
+  const int pos0 = SEL ? sel_pos(p, PAGED, seq) : PAGED ? p.seq_len[seq] - T : *p.pos0;
 
   // Local rows to attend (n) and the tiles of this CTA. Tiles are numbered over the local rows of the
   // sequence (tile t = rows 64 t ..). A CTA owns the `n_static` tiles from `t_first` on; one sequence
@@ -218,7 +224,15 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   if (p.n_local >= 0) n = min(n, p.n_local);
   n = max(0, min(n, p.n_ctx));
   int t_first, n_static, n_end, pool0, ntiles_all;
-  if (PAGED) {
+  int* const list = (int*)(sgen + L::OFF_LIST);
+  if (SEL) {
+    t_first = n_static = ntiles_all = pool0 = 0;
+    n_end = n;
+    if (warp == 0) {
+      const int c = collect_blocks(p, PAGED, seq, kh, ch * p.chunk_len, min(p.sel_k, (ch + 1) * p.chunk_len), n, list);
+      if (lane == 0) list[SEL_CHUNK] = c;
+    }
+  } else if (PAGED) {
     const int c0 = min(n, ch * p.chunk_len), c1 = min(n, c0 + p.chunk_len);
     t_first = c0 / TILE;
     n_static = (c1 - c0 + TILE - 1) / TILE;
@@ -236,7 +250,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   const bool has_pool = !PAGED && pool0 < ntiles_all;
   float* out = p.part + (((size_t)seq * p.nkvh + kh) * p.nch + ch) * MAXR * PROW;
 
-  if (n_static == 0 && !has_pool) {
+  if (!SEL && n_static == 0 && !has_pool) {
     // Nothing to do. The merge reads only the partials that hold something (filled_chunks; with pages the chunks
     // that a sequence has): anything else it reads is the neutral partial (src/attn.cu:117-120).
     if (!PAGED && ch < filled_chunks(n, p.nch))
@@ -245,6 +259,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   }
 
   __syncthreads();
+  if (SEL) n_static = list[SEL_CHUNK];  // may be 0: then no tile is loaded, and the partial is the neutral one
   if (tid == 0) stamp(1);
 
   // Row of the K/V tensors at which tile t starts.
@@ -252,7 +267,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
     int row = kh * p.n_ctx + t * TILE;
     if (PAGED) {  // a tile never straddles a page (64 | 256)
       const int pp = t * TILE;
-      int pg = p.page_table[(size_t)seq * p.max_pages + pp / Q27B_PAGE];
+      int pg = p.page_table[(size_t)(SEL ? seq / p.sel_T : seq) * p.max_pages + pp / Q27B_PAGE];
       if (pg < 0 || pg >= p.n_pages) {  // never read outside the pool: flag it and read page 0
         atomicOr(p.status, ST_BAD_PAGE);
         pg = 0;
@@ -286,6 +301,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   // memory (8 entries per group, entry j mod 8), which the loader fills three tiles ahead.
   auto next_tile = [&](int j) {
     const int i = grp + NG * j;
+    if (SEL) return i < n_static ? list[i] : -1;
     if (i < n_static) return t_first + i;
     if (!has_pool) return -1;
     const int t = pool0 + atomicAdd(p.sched + kh, 1);
@@ -791,6 +807,17 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
     }
   }
   bar_sync(BAR_PVALL, 128 * NG);
+  if (SEL) {  // [row][chunk]: row = (sequence, token, head)
+    const size_t row0 = (size_t)seq * p.nqh + kh * GQA;
+    for (int i = tid - PV0; i < GQA * (PROW / 2); i += 128 * NG) {
+      const int r = i / (PROW / 2), c = i % (PROW / 2);
+      const uint2 v = lds64(sStage + r * (PROW * 4) + 8 * c);
+      const size_t at = (row0 + r) * p.nch + ch;
+      if (c == 0) p.part_ml[at] = make_float2(__uint_as_float(v.x), __uint_as_float(v.y));
+      else *(uint2*)(p.part_o + at * AD + 2 * (c - 1)) = v;
+    }
+    return;
+  }
   for (int i = tid - PV0; i < R * PROW / 4; i += 128 * NG) ((uint4*)out)[i] = lds128(sStage + 16 * i);  // R is a multiple of 6
   if (tid == PV0) stamp(7);
 }
@@ -807,6 +834,15 @@ int launch_ws_nt(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap
     Q27B_CK(launch_step(decode_ws_kernel<NT, true, NG>, grid, dim3(Lay<NG>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
   else
     Q27B_CK(launch_step(decode_ws_kernel<NT, false, NG>, grid, dim3(Lay<NG>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
+  return Q27B_OK;
+}
+
+template <bool PAGED, int NG>
+int blocks_attr() {
+  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               NG == 1 ? SPREAD_SMEM_BYTES : Lay<NG>::SEL_SMEM_BYTES));
+  if (NG == 1)
+    Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, true>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
   return Q27B_OK;
 }
 
@@ -857,6 +893,35 @@ int launch_decode_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtenso
   if (nt == 1) return launch_ws_nt<1, 2>(kv, ks, vv, vs, p, paged, nseq, s);
   if (nt == 2) return launch_ws_nt<2, 2>(kv, ks, vv, vs, p, paged, nseq, s);
   return launch_ws_nt<3, 2>(kv, ks, vv, vs, p, paged, nseq, s);
+}
+
+int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                     const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups) {
+  static bool attr[64] = {};
+  static std::mutex attr_mu;
+  int dev;
+  Q27B_CK(cudaGetDevice(&dev));
+  {
+    std::lock_guard<std::mutex> lock(attr_mu);
+    if (!attr[dev]) {
+      if (int rc = blocks_attr<false, 2>()) return rc;
+      if (int rc = blocks_attr<true, 2>()) return rc;
+      if (int rc = blocks_attr<false, 1>()) return rc;
+      if (int rc = blocks_attr<true, 1>()) return rc;
+      attr[dev] = true;
+    }
+  }
+  const dim3 grid(p.nch, p.nkvh, nseq);
+  const bool paged = p.page_table != nullptr;
+  if (groups == WsGroups::TWO) {
+    auto* k = paged ? decode_ws_kernel<1, true, 2, true> : decode_ws_kernel<1, false, 2, true>;
+    Q27B_CK(launch_step(k, grid, dim3(Lay<2>::THREADS), Lay<2>::SEL_SMEM_BYTES, s, *kv, *ks, *vv, *vs, p));
+  } else {
+    auto* k = paged ? decode_ws_kernel<1, true, 1, true> : decode_ws_kernel<1, false, 1, true>;
+    const int smem = groups == WsGroups::SPREAD ? SPREAD_SMEM_BYTES : Lay<1>::SEL_SMEM_BYTES;
+    Q27B_CK(launch_step(k, grid, dim3(Lay<1>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
+  }
+  return Q27B_OK;
 }
 
 }  // namespace q27b
