@@ -15,32 +15,56 @@ namespace q27b {
 namespace {
 
 // Merges the partials of a row, applies the gate and writes f16, or q8_1. One CTA a row, four groups of 64 threads that
-// take every fourth partial; a row without a visible position is 0.
+// take every fourth partial, the first ten of each requested before the maxima are known; a row without a visible position
+// is 0.
+constexpr int MERGE_PRE = 10;
+
 __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p) {
   __shared__ float4 sa[3][64];
-  __shared__ float sl[4];
+  __shared__ float sl[4], sm[8];
   const size_t row = blockIdx.x;
-  const int grp = threadIdx.x >> 6, c = threadIdx.x & 63;
-  pdl_wait();
-  pdl_trigger();
-  const float2* ml = p.part_ml + row * p.nsplit;
+  const int tid = threadIdx.x, grp = tid >> 6, c = tid & 63;
   int np = p.nsplit;  // partials that were written
+  // The split kernel ran right before and lets its dependents start only when everything before it has completed: what it does
+  // not write may be read before the wait.
   if (!p.sel) {
     const int b = (int)(row / ((size_t)p.c.T * p.c.nkvh * GQA)), ntot = tree_tiles(min(first_pos(p.c, b) + p.c.T, p.c.n_ctx));
     np = ntot ? (ntot - 1) / tree_share(p, ntot) + 1 : 0;
   }
+  const float4 g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c);
+  pdl_wait();
+  pdl_trigger();
+  const float2* ml = p.part_ml + row * p.nsplit;
+  const float* po = p.part_o + row * p.nsplit * AD + 4 * c;
+  float4 pre[MERGE_PRE];
+  float2 pml[MERGE_PRE];
+#pragma unroll
+  for (int i = 0; i < MERGE_PRE; i++)
+    if (grp + 4 * i < np) {
+      pre[i] = *(const float4*)(po + (size_t)(grp + 4 * i) * AD);
+      pml[i] = ml[grp + 4 * i];
+    }
   float M = M_INIT;
-  for (int z = 0; z < np; z++) M = fmaxf(M, ml[z].x);
+  for (int z = tid; z < np; z += 256) M = fmaxf(M, ml[z].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if ((tid & 31) == 0) sm[tid >> 5] = M;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
   float L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int z = grp; z < np; z += 4) {
-    const float2 v = ml[z];
-    if (v.y == 0.f) continue;  // holds nothing
+  auto add = [&](const float2& v, const float4& x) {
+    if (v.y == 0.f) return;  // holds nothing
     const float f = ex2((v.x - M) * LOG2E);
-    const float4 x = *(const float4*)(p.part_o + (row * p.nsplit + z) * AD + 4 * c);
     L += v.y * f;
     A.x += x.x * f, A.y += x.y * f, A.z += x.z * f, A.w += x.w * f;
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < MERGE_PRE; i++)
+    if (grp + 4 * i < np) add(pml[i], pre[i]);
+#pragma unroll 4
+  for (int z = grp + 4 * MERGE_PRE; z < np; z += 4) add(ml[z], *(const float4*)(po + (size_t)z * AD));
   if (grp > 0) sa[grp - 1][c] = A;
   if (c == 0) sl[grp] = L;
   __syncthreads();
@@ -52,7 +76,6 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p) {
     L += sl[k + 1];
   }
   const float inv = L == 0.f ? 0.f : 1.0f / L;
-  const float4 g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c);
   float y[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
   const float gv[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll

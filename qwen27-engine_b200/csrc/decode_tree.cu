@@ -12,8 +12,12 @@
 // may see (past the sequence, on a page that does not exist) are cleared on the way to the tensor core, and drafted V
 // chunks of 16 dims that are not finite are cleared and remembered: the rows that see such a draft get NaN in these dims.
 //
-// Warps 0-7 softmax (two threads a row, 32 columns of a tile each), warp 8 TMA producer, warp 9 issues the Q K^T MMAs, warp
-// 10 the P V MMAs; on a q8_0 cache warps 11-14 turn K and 15-18 V from int8 into f16 operands.
+// Warps 0-7 softmax (two threads a row, 32 columns of a tile each), warp 8 issues the Q K^T MMAs, warp 9 the P V MMAs. f16
+// cache: warp 10 brings the tiles by TMA as the tensor core reads them. q8_0 cache: warps 10-13 turn K and 14-17 V into f16
+// operands, from registers that they load straight from the cache, a tile ahead (and three tiles ahead into L2): through shared
+// memory, which 64 KB of operands a tile written and read again keep busy already, the int8 tile would cost another 68 KB.
+// TMEM: columns 0-255 O (f32), 256-383 two S buffers of 64 columns (f32), 384-511 the Q tile. (P over the scores it was made of
+// saves a store and a load of shared memory, but the next Q K^T then waits for P V: 102 us behind 150,000.)
 #include "cache_ref.h"
 #include "decode_rows.h"
 #include "f16_tile.cuh"
@@ -25,29 +29,23 @@ namespace {
 
 constexpr int QT = TREE_ROWS;    // query rows per CTA
 constexpr float TAU = 5.0f;
-constexpr int P_BYTES = QT * 128;           // f16 P: [128][64 positions]
 constexpr int NWG = 2, CW = PT / NWG, OW = AD / NWG;  // softmax threads per row; their columns of a tile and of O
-constexpr int NSW = 4 * NWG, TMA_WARP = NSW, MMA_WARP = NSW + 1, PV_WARP = NSW + 2, KCONV_WARP0 = NSW + 3, VCONV_WARP0 = NSW + 7;
-constexpr int N_CONV_WARPS = 4;
-enum { B_QFULL = 0, B_KFULL = 1, B_KEMPTY = 4, B_VFULL = 7, B_VEMPTY = 10, B_SFULL = 13, B_SEMPTY = 15, B_PFULL = 17, B_PEMPTY = 18, B_ODONE = 19,
-       B_RKFULL = 20, B_RKEMPTY = 22, B_RVFULL = 24, B_RVEMPTY = 26, NBAR = 28 };
-template <bool Q8>
-struct Lay {
-  static constexpr int NKF = Q8 ? 2 : 3;                   // f16 K buffers, and as many f16 V buffers
-  static constexpr int OFF_K = 0;
-  static constexpr int OFF_V = OFF_K + NKF * KV_BYTES;
-  static constexpr int OFF_P = OFF_V + NKF * KV_BYTES;
-  static constexpr int OFF_RAW = OFF_P + P_BYTES;          // q8_0: K stage 0, 1, V stage 0, 1
-  static constexpr int OFF_XCH = OFF_RAW + (Q8 ? 4 * RAW_BYTES : 0);  // [tile parity][NWG][128] f32
-  static constexpr int OFF_BAR = OFF_XCH + 2 * NWG * QT * 4;
-  static constexpr int OFF_BAD = OFF_BAR + NBAR * 8;       // [16 chunks of 16 dims][2 words]: drafts whose V chunk is not finite
-  static constexpr int OFF_SKIP = OFF_BAD + 16 * 8;        // [TREE_MAX_SHARE / 32] words: tiles on pages that do not exist
-  static constexpr int OFF_MISC = OFF_SKIP + TREE_MAX_SHARE / 8;
-  static constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
-  static constexpr int THREADS = (NSW + 3 + (Q8 ? 2 * N_CONV_WARPS : 0)) * 32;
-  static_assert(OFF_P % 1024 == 0 && OFF_RAW % 1024 == 0 && RAW_BYTES % 1024 == 0, "swizzled tiles need 1024-byte alignment");
-  static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
-};
+constexpr int NSW = 4 * NWG, MMA_WARP = NSW, PV_WARP = NSW + 1, TMA_WARP = NSW + 2, KCONV_WARP0 = NSW + 2, VCONV_WARP0 = NSW + 6;
+constexpr int N_CONV_WARPS = 4, NK = 3, NV = 2, NP = 2;  // f16 K and V buffers, buffers of P
+enum { B_QFULL = 0, B_KFULL = 1, B_KEMPTY = 4, B_VFULL = 7, B_VEMPTY = 10, B_SFULL = 13, B_SEMPTY = 15, B_PFULL = 17, B_PVDONE = 19, B_ODONE = 21, NBAR = 22 };
+// Shared memory
+constexpr int OFF_K = 0;
+constexpr int OFF_V = OFF_K + NK * KV_BYTES;
+constexpr int P_BYTES = QT * 128;                         // f16 P: [128][64 positions]; first the Q tile on its way to tensor memory
+constexpr int OFF_P = OFF_V + NV * KV_BYTES;
+constexpr int OFF_XCH = OFF_P + NP * P_BYTES;                  // [tile parity][NWG][128] f32
+constexpr int OFF_BAR = OFF_XCH + 2 * NWG * QT * 4;
+constexpr int OFF_BAD = OFF_BAR + NBAR * 8;               // [16 chunks of 16 dims][2 words]: drafts whose V chunk is not finite
+constexpr int OFF_SKIP = OFF_BAD + 16 * 8;                // [TREE_MAX_SHARE / 32] words: tiles on pages that do not exist
+constexpr int OFF_MISC = OFF_SKIP + TREE_MAX_SHARE / 8;
+constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
+static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
+constexpr int threads(bool q8) { return (NSW + 2 + (q8 ? 2 * N_CONV_WARPS : 1)) * 32; }
 constexpr uint32_t TMEM_COLS = 512;
 constexpr uint32_t TM_O = 0, TM_S = 256, TM_Q = 384;  // O f32 256 columns, S 2 x 64 f32, Q 128 columns of f16 pairs
 constexpr uint32_t IDESC_QK = umma_idesc(1, 0, 0, 0, 0, QT, PT);   // f32 += f16 * f16, both K-major, M128 N64
@@ -76,28 +74,35 @@ __device__ __noinline__ void clean_v_row(uint8_t* vrow, int r, int sg, int zone,
   }
 }
 
+// 16 bytes of the cache, read once.
+__device__ __forceinline__ uint4 load16(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 template <bool Q8, bool PAGED>
-__global__ void __launch_bounds__(Lay<Q8>::THREADS, 1)
-tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-            const __grid_constant__ CUtensorMap tm_ks, const __grid_constant__ CUtensorMap tm_vs, const RowsParams p) {
-  using LY = Lay<Q8>;
-  constexpr int NKF = LY::NKF, OFF_K = LY::OFF_K, OFF_V = LY::OFF_V, OFF_P = LY::OFF_P, OFF_RAW = LY::OFF_RAW, OFF_XCH = LY::OFF_XCH;
-  constexpr bool ROOM = LY::THREADS <= 384;  // registers for more loads in flight: 168 a thread; with 19 warps 96
+__global__ void __launch_bounds__(threads(Q8), 1)
+tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const RowsParams p) {
+  constexpr int THREADS = threads(Q8);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* sgen = smem_raw + (sbase - smem_u32(smem_raw));
-  uint64_t* bar = (uint64_t*)(sgen + LY::OFF_BAR);
-  uint32_t* bad = (uint32_t*)(sgen + LY::OFF_BAD);
-  uint32_t* skip = (uint32_t*)(sgen + LY::OFF_SKIP);
-  uint32_t* tmem_slot = (uint32_t*)(sgen + LY::OFF_MISC);
-  volatile int* abort_flag = (volatile int*)(sgen + LY::OFF_MISC + 4);
+  uint64_t* bar = (uint64_t*)(sgen + OFF_BAR);
+  uint32_t* bad = (uint32_t*)(sgen + OFF_BAD);
+  uint32_t* skip = (uint32_t*)(sgen + OFF_SKIP);
+  uint32_t* tmem_slot = (uint32_t*)(sgen + OFF_MISC);
+  volatile int* abort_flag = (volatile int*)(sgen + OFF_MISC + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int T = p.c.T, nkvh = p.c.nkvh, nqh = nkvh * GQA, z = blockIdx.x, kh = blockIdx.y % nkvh, row0 = (blockIdx.y / nkvh) * QT,
             b = blockIdx.z;
+  // Softmax warps q, q + 4 have rows 32 q ..; those past the last row have nothing to do (what the tensor core makes of their rows
+  // of Q and P reaches no other row).
+  const int rows_here = T * GQA - row0, n_active = NWG * min(4, (rows_here + 31) / 32);
 
   // What needs no memory of the call runs while the previous kernel of the stream drains.
   if (tid == 0) {
-    mbar_init(&bar[B_QFULL], NSW);
+    mbar_init(&bar[B_QFULL], n_active);
     for (int s = 0; s < 3; s++) {
       mbar_init(&bar[B_KFULL + s], Q8 ? N_CONV_WARPS : 1);  // q8_0: the converter warps fill the buffers
       mbar_init(&bar[B_KEMPTY + s], 1);
@@ -106,22 +111,18 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&bar[B_SFULL + s], 1);
-      mbar_init(&bar[B_SEMPTY + s], NSW);
-      mbar_init(&bar[B_RKFULL + s], 1);
-      mbar_init(&bar[B_RKEMPTY + s], N_CONV_WARPS);
-      mbar_init(&bar[B_RVFULL + s], 1);
-      mbar_init(&bar[B_RVEMPTY + s], N_CONV_WARPS);
+      mbar_init(&bar[B_SEMPTY + s], n_active);
     }
-    mbar_init(&bar[B_PFULL], NSW);
-    mbar_init(&bar[B_PEMPTY], 1);
+    for (int s = 0; s < NP; s++) {
+      mbar_init(&bar[B_PFULL + s], n_active);
+      mbar_init(&bar[B_PVDONE + s], 1);
+    }
     mbar_init(&bar[B_ODONE], 1);
     *abort_flag = 0;
     mbar_fence_init();
-    tma_prefetch_desc(&tm_k);
-    tma_prefetch_desc(&tm_v);
-    if (Q8) {
-      tma_prefetch_desc(&tm_ks);
-      tma_prefetch_desc(&tm_vs);
+    if (!Q8) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
     }
   }
   if (tid < 32) bad[tid] = 0;
@@ -140,7 +141,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   tc_fence_before();
   __syncthreads();
   if (PAGED) {  // the pages of this share: what lies on one that is none is not visible
-    for (int j = tid; j < nt; j += LY::THREADS)
+    for (int j = tid; j < nt; j += THREADS)
       if (cache_row(p.c, b, kh, (it0 + j) * PT) < 0) atomicOr(&skip[j >> 5], 1u << (j & 31));
     __syncthreads();
   }
@@ -148,7 +149,9 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   const uint32_t tmem = *tmem_slot;
   auto skipped = [&](int j) { return PAGED && ((((volatile uint32_t*)skip)[j >> 5] >> (j & 31)) & 1); };
 
-  if (warp < NSW) {
+  if (warp < NSW && (warp & 3) >= n_active / NWG) {
+    // no rows
+  } else if (warp < NSW) {
     // ================================================================ softmax warps
     const int wg = warp >> 2, q = warp & 3;
     const int r = q * 32 + lane;       // query row = TMEM lane
@@ -157,13 +160,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     const uint32_t tlane = tmem + ((uint32_t)(q * 32) << 16);
     // output row of row gr of the KV head
     auto out_row = [&](int gr) { return ((size_t)b * T + gr / GQA) * nqh + kh * GQA + gr % GQA; };
-    uint64_t mine = t < T ? p.mask[(size_t)b * T + t] : 0;
-    if (T < 64) mine &= ((uint64_t)1 << T) - 1;
     {
-      constexpr int LD = ROOM ? 2 : 1;  // turns whose loads are requested together
       // Q tile -> tensor memory, lane = row, column c = dims 2c, 2c + 1 as f16: this warp writes dims OW wg .. of its 32
       // rows, scaled and rounded; rows past 6 T are zero. 32 dims at a time, loaded with eight lanes to 128 contiguous bytes of
-      // a row and turned to a row per thread in the P buffer (64 bytes a row, 16-byte chunk c of row r at c ^ (r / 2 % 4)).
+      // a row and turned to a row per thread in shared memory (64 bytes a row, 16-byte chunk c of row r at c ^ (r / 2 % 4)).
+      constexpr int LD = 2;  // turns whose loads are requested together
       uint8_t* stage = sgen + OFF_P + warp * 2048;
       static_assert(NSW * 2048 <= P_BYTES, "staging of the Q tile");
 #pragma unroll 1
@@ -202,6 +203,8 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[B_QFULL]);
     }
+    uint64_t mine = t < T ? p.mask[(size_t)b * T + t] : 0;
+    if (T < 64) mine &= ((uint64_t)1 << T) - 1;
 
     const int col0 = wg * CW;          // this thread's positions of a tile
     float m_run = M_INIT, m_ref = M_INIT;
@@ -225,7 +228,6 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar[B_SEMPTY + slot]);  // the buffer is in registers: it can be overwritten
-
       // Columns of the tile that this row sees; only tiles that reach past the prefix (or lie on no page) have others.
       if (p_tile + PT > zone || skipped(j)) {
         const int j0 = p_tile - first;  // the draft in column 0
@@ -262,7 +264,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
         l2 = mul2(l2, pack2(f, f));
         if (j > 0) {
           // O holds the sum of tiles < j once the P V of tile j-1 has completed
-          mbar_wait(&bar[B_PEMPTY], (j - 1) & 1, abort_flag, p.c.status);
+          mbar_wait(&bar[B_PVDONE + (slot ^ 1)], ((j - 1) >> 1) & 1, abort_flag, p.c.status);
           tc_fence_after();
           rescale_o_f16(tlane + TM_O + wg * OW, f, OW / 32);
           tc_wait_st();
@@ -271,8 +273,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       }
 
       // P = exp(s - m_ref): f32 row sum, f16 for the P V MMA (16-byte chunks CW/8 wg .. of the row)
-      mbar_wait(&bar[B_PEMPTY], (j & 1) ^ 1, abort_flag, p.c.status);  // P V of tile j-1 has read the buffer
-      uint8_t* sP = sgen + OFF_P;
+      mbar_wait(&bar[B_PVDONE + slot], ((j >> 1) & 1) ^ 1, abort_flag, p.c.status);  // P V of tile j-2 has read the buffer
       const float nmb = -m_ref * LOG2E;
       const uint64_t nmb2 = pack2(nmb, nmb);
 #pragma unroll
@@ -286,18 +287,18 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
           l2 = add2(l2, pack2(e0, e1));
           w[k] = pack_h2(e0, e1);
         }
-        *(uint4*)(sP + swz128(r, CW / 8 * wg + c)) = make_uint4(w[0], w[1], w[2], w[3]);
+        *(uint4*)(sgen + OFF_P + slot * P_BYTES + swz128(r, CW / 8 * wg + c)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
       if (!Q8 && p_tile + PT > zone) {  // f16 cache: V lies in the operand buffer as it came (the converters do this for q8_0)
-        const int vb = j % NKF;
-        mbar_wait(&bar[B_VFULL + vb], (j / NKF) & 1, abort_flag, p.c.status);
-        static_assert(32 * NSW == 4 * PT, "a thread per (segment, row)");
-        const int sg = tid >> 6, row = tid & 63;
-        clean_v_row(sgen + OFF_V + vb * KV_BYTES + sg * SEGK + row * 128, row, sg, zone - p_tile, n_end - p_tile, p_tile + row - first, bad);
+        const int vb = j % NV;
+        mbar_wait(&bar[B_VFULL + vb], (j / NV) & 1, abort_flag, p.c.status);
+        for (int u = (wg * (n_active / NWG) + q) * 32 + lane; u < 4 * PT; u += 32 * n_active)  // (segment, row)
+          clean_v_row(sgen + OFF_V + vb * KV_BYTES + (u >> 6) * SEGK + (u & 63) * 128, u & 63, u >> 6, zone - p_tile, n_end - p_tile,
+                      p_tile + (u & 63) - first, bad);
       }
       fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[B_PFULL]);
+      if (lane == 0) mbar_arrive(&bar[B_PFULL + slot]);
     }
 
     // ---- epilogue: the unnormalised partial of this share
@@ -341,92 +342,6 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       __syncwarp();
     }
     tc_fence_before();
-  } else if (warp == TMA_WARP) {
-    // ================================================================ TMA producer
-    if (lane == 0) {
-#pragma unroll 1
-      for (int j = 0; j < nt; j++) {
-        const int pos = (it0 + j) * PT;
-        int row = kh * p.c.n_ctx + pos;
-        if (PAGED)  // a tile never straddles a page; one that lies on none is fetched from the pool's first page and not seen
-          row = skipped(j) ? 0 : (p.c.page_table[(size_t)b * p.c.max_pages + pos / Q27B_PAGE] * nkvh + kh) * Q27B_PAGE + pos % Q27B_PAGE;
-        if constexpr (Q8) {
-          const int st = j & 1, ph = (j >> 1) & 1;  // raw stages
-          uint8_t* kr = sgen + OFF_RAW + st * RAW_BYTES;
-          uint8_t* vr = sgen + OFF_RAW + (2 + st) * RAW_BYTES;
-          mbar_wait(&bar[B_RKEMPTY + st], ph ^ 1, abort_flag, p.c.status);
-          mbar_expect_tx(&bar[B_RKFULL + st], RAW_BYTES);
-          tma_load_2d(kr, &tm_k, 0, row, &bar[B_RKFULL + st]);
-          tma_load_2d(kr + PT * 128, &tm_k, 128, row, &bar[B_RKFULL + st]);
-          tma_load_2d(kr + 2 * PT * 128, &tm_ks, 0, row, &bar[B_RKFULL + st]);
-          mbar_wait(&bar[B_RVEMPTY + st], ph ^ 1, abort_flag, p.c.status);
-          mbar_expect_tx(&bar[B_RVFULL + st], RAW_BYTES);
-          tma_load_2d(vr, &tm_v, 0, row, &bar[B_RVFULL + st]);
-          tma_load_2d(vr + PT * 128, &tm_v, 128, row, &bar[B_RVFULL + st]);
-          tma_load_2d(vr + 2 * PT * 128, &tm_vs, 0, row, &bar[B_RVFULL + st]);
-        } else {
-          const int st = j % NKF, ph = (j / NKF) & 1;
-          uint8_t* ks = sgen + OFF_K + st * KV_BYTES;
-          uint8_t* vs = sgen + OFF_V + st * KV_BYTES;
-          mbar_wait(&bar[B_KEMPTY + st], ph ^ 1, abort_flag, p.c.status);
-          mbar_expect_tx(&bar[B_KFULL + st], KV_BYTES);
-#pragma unroll
-          for (int sg = 0; sg < 4; sg++) tma_load_2d(ks + sg * SEGK, &tm_k, sg * 128, row, &bar[B_KFULL + st]);
-          mbar_wait(&bar[B_VEMPTY + st], ph ^ 1, abort_flag, p.c.status);
-          mbar_expect_tx(&bar[B_VFULL + st], KV_BYTES);
-#pragma unroll
-          for (int sg = 0; sg < 4; sg++) tma_load_2d(vs + sg * SEGK, &tm_v, sg * 128, row, &bar[B_VFULL + st]);
-        }
-      }
-    }
-  } else if (Q8 && warp >= KCONV_WARP0) {
-    // ================================================================ converter warps (q8_0 cache)
-    const bool is_v = warp >= VCONV_WARP0;
-    const int ct = tid - (is_v ? VCONV_WARP0 : KCONV_WARP0) * 32;
-    const int b_rfull = is_v ? B_RVFULL : B_RKFULL, b_rempty = is_v ? B_RVEMPTY : B_RKEMPTY;
-    const int b_full = is_v ? B_VFULL : B_KFULL, b_empty = is_v ? B_VEMPTY : B_KEMPTY;
-    const ConvAddr ca = conv_addr(ct);
-#pragma unroll 1
-    for (int j = 0; j < nt; j++) {
-      const int st = j & 1, fb = j % NKF, p_tile = (it0 + j) * PT;
-      mbar_wait(&bar[b_rfull + st], (j >> 1) & 1, abort_flag, p.c.status);
-      mbar_wait(&bar[b_empty + fb], ((j / NKF) & 1) ^ 1, abort_flag, p.c.status);  // the MMAs of tile j-NKF have read the buffer
-      uint8_t* dst = sgen + (is_v ? OFF_V : OFF_K) + fb * KV_BYTES;
-      convert_q8_tile(sgen + OFF_RAW + ((is_v ? 2 : 0) + st) * RAW_BYTES, dst, ca, is_v ? (skipped(j) ? 0 : n_end - p_tile) : PT);
-      if (is_v && p_tile + PT > zone) {  // drafted rows: see clean_v_row
-        asm volatile("bar.sync %0, %1;" ::"n"(1 + 4), "n"(32 * N_CONV_WARPS) : "memory");
-#pragma unroll 1
-        for (int u = ct; u < 4 * PT; u += 32 * N_CONV_WARPS)
-          clean_v_row(dst + (u >> 6) * SEGK + (u & 63) * 128, u & 63, u >> 6, zone - p_tile, skipped(j) ? 0 : n_end - p_tile,
-                      p_tile + (u & 63) - first, bad);
-      }
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&bar[b_full + fb]);
-        mbar_arrive(&bar[b_rempty + st]);
-      }
-    }
-  } else if (warp == PV_WARP) {
-    // ================================================================ P V issuer
-    if (lane == 0) {
-#pragma unroll 1
-      for (int j = 0; j < nt; j++) {
-        const int st = j % NKF, ph = (j / NKF) & 1;
-        mbar_wait(&bar[B_PFULL], j & 1, abort_flag, p.c.status);
-        mbar_wait(&bar[B_VFULL + st], ph, abort_flag, p.c.status);
-        tc_fence_after();
-#pragma unroll
-        for (int kk = 0; kk < PT / 16; kk++) {
-          const uint64_t da = umma_desc_sw128(sbase + OFF_P + kk * 32, 16, 1024);
-          const uint64_t db = umma_desc_sw128(sbase + OFF_V + st * KV_BYTES + kk * 2048, SEGK, 1024);
-          tc_mma_f16(tmem + TM_O, da, db, IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
-        }
-        tc_commit(&bar[B_PEMPTY]);
-        tc_commit(&bar[B_VEMPTY + st]);
-      }
-      tc_commit(&bar[B_ODONE]);
-    }
   } else if (warp == MMA_WARP) {
     // ================================================================ Q K^T issuer
     if (lane == 0) {
@@ -435,7 +350,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
 #pragma unroll 1
       for (int j = 0; j < nt; j++) {
         const int ss = j & 1, sph = (j >> 1) & 1;                         // S buffer
-        const int st = j % NKF, ph = (j / NKF) & 1;                       // K buffer
+        const int st = j % NK, ph = (j / NK) & 1;                         // K buffer
         mbar_wait(&bar[B_KFULL + st], ph, abort_flag, p.c.status);
         mbar_wait(&bar[B_SEMPTY + ss], sph ^ 1, abort_flag, p.c.status);
         tc_fence_after();
@@ -447,6 +362,138 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
         tc_commit(&bar[B_SFULL + ss]);
         tc_commit(&bar[B_KEMPTY + st]);
       }
+    }
+  } else if (warp == PV_WARP) {
+    // ================================================================ P V issuer
+    if (lane == 0) {
+#pragma unroll 1
+      for (int j = 0; j < nt; j++) {
+        const int st = j % NV, ph = (j / NV) & 1, pb = j & 1;
+        mbar_wait(&bar[B_PFULL + pb], (j >> 1) & 1, abort_flag, p.c.status);
+        mbar_wait(&bar[B_VFULL + st], ph, abort_flag, p.c.status);
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < PT / 16; kk++) {
+          const uint64_t db = umma_desc_sw128(sbase + OFF_V + st * KV_BYTES + kk * 2048, SEGK, 1024);
+          const uint64_t da = umma_desc_sw128(sbase + OFF_P + pb * P_BYTES + kk * 32, 16, 1024);
+          tc_mma_f16(tmem + TM_O, da, db, IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
+        }
+        tc_commit(&bar[B_PVDONE + pb]);
+        tc_commit(&bar[B_VEMPTY + st]);
+      }
+      tc_commit(&bar[B_ODONE]);
+    }
+  } else if constexpr (!Q8) {
+    // ================================================================ TMA producer (f16 cache)
+    if (lane == 0) {
+#pragma unroll 1
+      for (int j = 0; j < nt; j++) {
+        const int row = kh * p.c.n_ctx + (it0 + j) * PT, kb = j % NK, vb = j % NV;
+        uint8_t* ks = sgen + OFF_K + kb * KV_BYTES;
+        uint8_t* vs = sgen + OFF_V + vb * KV_BYTES;
+        mbar_wait(&bar[B_KEMPTY + kb], ((j / NK) & 1) ^ 1, abort_flag, p.c.status);
+        mbar_expect_tx(&bar[B_KFULL + kb], KV_BYTES);
+#pragma unroll
+        for (int sg = 0; sg < 4; sg++) tma_load_2d(ks + sg * SEGK, &tm_k, sg * 128, row, &bar[B_KFULL + kb]);
+        mbar_wait(&bar[B_VEMPTY + vb], ((j / NV) & 1) ^ 1, abort_flag, p.c.status);
+        mbar_expect_tx(&bar[B_VFULL + vb], KV_BYTES);
+#pragma unroll
+        for (int sg = 0; sg < 4; sg++) tma_load_2d(vs + sg * SEGK, &tm_v, sg * 128, row, &bar[B_VFULL + vb]);
+      }
+    }
+  } else {
+    // ================================================================ converter warps (q8_0 cache)
+    // Thread ct: 16 dims (chunk c16) of rows a.row0, a.row0 + 8, .. of every tile, in registers a tile ahead.
+    const bool is_v = warp >= VCONV_WARP0;
+    const int ct = tid - (is_v ? VCONV_WARP0 : KCONV_WARP0) * 32, c16 = (ct & 3) + 4 * ((ct >> 3) & 3);
+    const int b_full = is_v ? B_VFULL : B_KFULL, b_empty = is_v ? B_VEMPTY : B_KEMPTY;
+    const ConvAddr a = conv_addr(ct);
+    const uint8_t* vals = (const uint8_t*)(is_v ? p.vcache : p.kcache);
+    const uint8_t* scales = vals + cache_rows(p.c) * AD;
+    // first row of tile j, and how many of its rows are there (past them, and on no page, nothing is read)
+    auto tile_row = [&](int j) -> int64_t {
+      const int pos = (it0 + j) * PT;
+      if (!PAGED) return (int64_t)kh * p.c.n_ctx + pos;
+      if (skipped(j)) return 0;
+      return ((int64_t)p.c.page_table[(size_t)b * p.c.max_pages + pos / Q27B_PAGE] * nkvh + kh) * Q27B_PAGE + pos % Q27B_PAGE;
+    };
+    auto tile_rows = [&](int j) { return skipped(j) ? 0 : min(PT, n_end - (it0 + j) * PT); };
+    uint4 x[8];
+    uint32_t d[8];
+    const uint8_t *src = nullptr, *ssrc = nullptr;  // this thread's first chunk of the tile that is fetched, and its scale
+    int there = 0;                                  // rows of that tile from a.row0 on
+    auto aim = [&](int j) {
+      const int64_t row = tile_row(j) + a.row0;
+      src = vals + row * AD + 16 * c16;
+      ssrc = scales + row * 16 + (c16 >> 1) * 2;
+      there = tile_rows(j) - a.row0;
+    };
+    // Rows that are not there: the bytes of the tile's first row (or the pool's) times 0.
+    auto fetch = [&](int k, bool whole) {
+      const int r = whole || 8 * k < there ? 8 * k : -a.row0;
+      x[k] = load16(src + r * AD);
+      d[k] = whole || 8 * k < there ? *(const uint16_t*)(ssrc + r * 16) : 0;
+    };
+    auto to_l2 = [&](int j) {
+      if (ct != 0 || j >= nt || tile_rows(j) <= 0) return;
+      const int64_t row = tile_row(j);
+      const uint32_t rows = (uint32_t)tile_rows(j);
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(vals + row * AD), "r"(rows * AD) : "memory");
+      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(scales + row * 16), "r"(rows * 16) : "memory");
+    };
+    // Item k of the tile in registers into the f16 buffer, and the same item of the next tile fetched in its place.
+    auto convert = [&](int k, uint8_t* dst, bool more, bool whole, int drafted) {
+      const __half2 dd = u32_as_h2(__byte_perm(d[k], d[k], 0x1010));
+      const uint32_t xw[4] = {x[k].x ^ 0x80808080u, x[k].y ^ 0x80808080u, x[k].z ^ 0x80808080u, x[k].w ^ 0x80808080u};
+      uint32_t o[8];
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        o[2 * w] = dq_pair(__byte_perm(xw[w], 0x64646464u, 0x4140), dd);
+        o[2 * w + 1] = dq_pair(__byte_perm(xw[w], 0x64646464u, 0x4342), dd);
+      }
+      if (more) fetch(k, whole);
+      if (drafted >= 0) {  // this row is a draft's
+        bool nf = false;
+#pragma unroll
+        for (int w = 0; w < 8; w++) nf |= not_finite(o[w]);
+        if (nf) {
+          atomicOr(&bad[2 * c16 + (drafted >> 5)], 1u << (drafted & 31));
+#pragma unroll
+          for (int w = 0; w < 8; w++) o[w] = 0;
+        }
+      }
+      *(uint4*)(dst + a.dst + k * 1024) = make_uint4(o[0], o[1], o[2], o[3]);
+      *(uint4*)(dst + (a.dst ^ 16u) + k * 1024) = make_uint4(o[4], o[5], o[6], o[7]);
+    };
+    aim(0);
+#pragma unroll
+    for (int k = 0; k < 8; k++) fetch(k, false);
+    to_l2(1);
+    to_l2(2);
+    const int nbuf = is_v ? NV : NK;
+    int fb = 0, ph = 1;
+#pragma unroll 1
+    for (int j = 0; j < nt; j++) {
+      const int p_tile = (it0 + j) * PT;
+      to_l2(j + 3);
+      const bool more = j + 1 < nt;
+      if (more) aim(j + 1);
+      mbar_wait(&bar[b_empty + fb], ph, abort_flag, p.c.status);  // the MMAs of the tile before it have read the buffer
+      uint8_t* dst = sgen + (is_v ? OFF_V : OFF_K) + fb * KV_BYTES;
+      if (more && tile_rows(j + 1) == PT && p_tile + PT <= zone) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) convert(k, dst, true, true, -1);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+          const int pos = p_tile + a.row0 + 8 * k;
+          convert(k, dst, more, false, is_v && pos >= zone && pos < n_end ? pos - first : -1);
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar[b_full + fb]);
+      if (++fb == nbuf) fb = 0, ph ^= 1;
     }
   }
 
@@ -461,7 +508,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
 
 template <bool Q8, bool PAGED>
 int tree_attr() {
-  Q27B_CK(cudaFuncSetAttribute(tree_kernel<Q8, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<Q8>::SMEM_BYTES));
+  Q27B_CK(cudaFuncSetAttribute(tree_kernel<Q8, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
   return Q27B_OK;
 }
 
@@ -481,24 +528,18 @@ int launch_tree(const RowsParams& p, cudaStream_t s) {
       attr[dev] = true;
     }
   }
-  CUtensorMap tk, tv, tks, tvs;
-  const uint64_t rows = cache_rows(p.c);
-  if (p.c.q8) {
-    if (int rc = q8_tmaps(p.kcache, rows, &tk, &tks)) return rc;
-    if (int rc = q8_tmaps(p.vcache, rows, &tv, &tvs)) return rc;
+  const dim3 grid(p.nsplit, p.c.nkvh * tree_row_tiles(p.c.T), p.c.B);
+  CUtensorMap tk = {}, tv = {};  // f16 only
+  if (p.c.page_table) {
+    Q27B_CK(launch_step(tree_kernel<true, true>, grid, dim3(threads(true)), SMEM_BYTES, s, tk, tv, p));
+  } else if (p.c.q8) {
+    Q27B_CK(launch_step(tree_kernel<true, false>, grid, dim3(threads(true)), SMEM_BYTES, s, tk, tv, p));
   } else {
+    const uint64_t rows = cache_rows(p.c);
     if (int rc = cached_tmap_2d(&tk, p.kcache, rows, 2 * AD, 2 * AD, 128, PT, true)) return rc;
     if (int rc = cached_tmap_2d(&tv, p.vcache, rows, 2 * AD, 2 * AD, 128, PT, true)) return rc;
-    tks = tk;  // not read
-    tvs = tv;
+    Q27B_CK(launch_step(tree_kernel<false, false>, grid, dim3(threads(false)), SMEM_BYTES, s, tk, tv, p));
   }
-  const dim3 grid(p.nsplit, p.c.nkvh * tree_row_tiles(p.c.T), p.c.B);
-  if (p.c.page_table)
-    Q27B_CK(launch_step(tree_kernel<true, true>, grid, dim3(Lay<true>::THREADS), Lay<true>::SMEM_BYTES, s, tk, tv, tks, tvs, p));
-  else if (p.c.q8)
-    Q27B_CK(launch_step(tree_kernel<true, false>, grid, dim3(Lay<true>::THREADS), Lay<true>::SMEM_BYTES, s, tk, tv, tks, tvs, p));
-  else
-    Q27B_CK(launch_step(tree_kernel<false, false>, grid, dim3(Lay<false>::THREADS), Lay<false>::SMEM_BYTES, s, tk, tv, tks, tvs, p));
   return Q27B_OK;
 }
 
