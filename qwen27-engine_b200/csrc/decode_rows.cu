@@ -14,44 +14,75 @@
 namespace q27b {
 namespace {
 
-// Merges the partials of a row, applies the gate and writes f16, or q8_1. One CTA a row, four groups of 64 threads that
-// take every fourth partial, the first ten of each requested before the maxima are known; a row without a visible position
-// is 0.
+// Merges the partials of a row, applies the gate and writes f16, or q8_1; a row without a visible position is 0. 64 threads to
+// a row, four dims each, or GROUPS times as many that take every GROUPS-th partial; the first ten of each are requested before the
+// maxima are known. Many rows have few partials each (a batch): four rows to a CTA of 256 threads then.
 constexpr int MERGE_PRE = 10;
 
-__global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p) {
-  __shared__ float4 sa[3][64];
+template <int GROUPS>
+__global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p, int64_t rows) {
+  constexpr int ROWS = 4 / GROUPS;  // of a CTA
+  __shared__ float4 sa[GROUPS > 1 ? GROUPS - 1 : 1][64];
   __shared__ float sl[4], sm[8];
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x, grp = tid >> 6, c = tid & 63;
-  int np = p.nsplit;  // partials that were written
+  const int tid = threadIdx.x, grp = GROUPS > 1 ? tid >> 6 : 0, c = tid & 63;
+  const size_t row = (size_t)blockIdx.x * ROWS + (GROUPS > 1 ? 0 : tid >> 6);
+  const bool mine = (int64_t)row < rows;
   // The split kernel ran right before and lets its dependents start only when everything before it has completed: what it does
   // not write may be read before the wait.
-  if (!p.sel) {
-    const int b = (int)(row / ((size_t)p.c.T * p.c.nkvh * GQA)), ntot = tree_tiles(min(first_pos(p.c, b) + p.c.T, p.c.n_ctx));
-    np = ntot ? (ntot - 1) / tree_share(p, ntot) + 1 : 0;
+  int b = 0, y = 0, r = 0, tiles = 0;  // tree: sequence, unit in it and row in that; its tiles
+  const int nqh = p.c.nkvh * GQA;
+  float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mine) {
+    g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c);
+    if (!p.sel) {
+      b = (int)(row / ((size_t)p.c.T * nqh));
+      const int h = (int)(row % nqh), gr = (int)(row / nqh % p.c.T) * GQA + h % GQA;
+      y = gr / TREE_ROWS * p.c.nkvh + h / GQA;
+      r = gr % TREE_ROWS;
+      tiles = tree_tiles(min(first_pos(p.c, b) + p.c.T, p.c.n_ctx));
+    }
   }
-  const float4 g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c);
   pdl_wait();
   pdl_trigger();
-  const float2* ml = p.part_ml + row * p.nsplit;
-  const float* po = p.part_o + row * p.nsplit * AD + 4 * c;
+  int np = 0;        // partials of the row: first, first + step, ..
+  size_t first = 0, step = 1;
+  if (mine && p.sel) {
+    np = p.nsplit;
+    first = row * p.nsplit;
+  } else if (mine && tiles > 0) {
+    const int units = p.c.nkvh * tree_row_tiles(p.c.T);
+    if (p.c.page_table) {
+      np = tree_parts(tiles, (int)p.plan[0]);
+      first = (size_t)p.plan[1 + b] * units + (size_t)y * np;
+    } else {
+      np = min(p.nsplit, tiles);
+      first = (size_t)y * p.nsplit;
+    }
+    first = first * TREE_ROWS + r;
+    step = TREE_ROWS;
+  }
+  const float2* ml = p.part_ml + first;
+  const float* po = p.part_o + first * AD + 4 * c;
   float4 pre[MERGE_PRE];
   float2 pml[MERGE_PRE];
 #pragma unroll
   for (int i = 0; i < MERGE_PRE; i++)
-    if (grp + 4 * i < np) {
-      pre[i] = *(const float4*)(po + (size_t)(grp + 4 * i) * AD);
-      pml[i] = ml[grp + 4 * i];
+    if (grp + GROUPS * i < np) {
+      pre[i] = *(const float4*)(po + (size_t)(grp + GROUPS * i) * step * AD);
+      pml[i] = ml[(size_t)(grp + GROUPS * i) * step];
     }
   float M = M_INIT;
-  for (int z = tid; z < np; z += 256) M = fmaxf(M, ml[z].x);
+  for (int z = GROUPS > 1 ? tid : c; z < np; z += 64 * GROUPS) M = fmaxf(M, ml[(size_t)z * step].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if ((tid & 31) == 0) sm[tid >> 5] = M;
   __syncthreads();
+  if (GROUPS > 1) {
 #pragma unroll
-  for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
+    for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
+  } else {
+    M = fmaxf(sm[tid >> 6 << 1], sm[(tid >> 6 << 1) + 1]);
+  }
   float L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](const float2& v, const float4& x) {
@@ -62,64 +93,61 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p) {
   };
 #pragma unroll
   for (int i = 0; i < MERGE_PRE; i++)
-    if (grp + 4 * i < np) add(pml[i], pre[i]);
+    if (grp + GROUPS * i < np) add(pml[i], pre[i]);
 #pragma unroll 4
-  for (int z = grp + 4 * MERGE_PRE; z < np; z += 4) add(ml[z], *(const float4*)(po + (size_t)z * AD));
-  if (grp > 0) sa[grp - 1][c] = A;
-  if (c == 0) sl[grp] = L;
-  __syncthreads();
-  if (grp > 0) return;
+  for (int z = grp + GROUPS * MERGE_PRE; z < np; z += GROUPS) add(ml[(size_t)z * step], *(const float4*)(po + (size_t)z * step * AD));
+  if (GROUPS > 1) {
+    if (grp > 0) sa[grp - 1][c] = A;
+    if (c == 0) sl[grp] = L;
+    __syncthreads();
+    if (grp > 0) return;
 #pragma unroll
-  for (int k = 0; k < 3; k++) {
-    const float4 x = sa[k][c];
-    A.x += x.x, A.y += x.y, A.z += x.z, A.w += x.w;
-    L += sl[k + 1];
+    for (int k = 0; k < GROUPS - 1; k++) {
+      const float4 x = sa[k][c];
+      A.x += x.x, A.y += x.y, A.z += x.z, A.w += x.w;
+      L += sl[k + 1];
+    }
   }
+  if (!mine) return;
   const float inv = L == 0.f ? 0.f : 1.0f / L;
-  float y[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
+  float out[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
   const float gv[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
-  for (int i = 0; i < 4; i++) y[i] *= 1.0f / (1.0f + expf(-gv[i]));
+  for (int i = 0; i < 4; i++) out[i] *= 1.0f / (1.0f + expf(-gv[i]));
   if (!p.xq) {
-    *(uint2*)((__half*)p.o + row * AD + 4 * c) = make_uint2(pack_h2(y[0], y[1]), pack_h2(y[2], y[3]));
+    *(uint2*)((__half*)p.o + row * AD + 4 * c) = make_uint2(pack_h2(out[0], out[1]), pack_h2(out[2], out[3]));
     return;
   }
   // q8_1 of 32 dims = eight lanes, as the merge of attn_decode writes it
-  float amax = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
+  float amax = fmaxf(fmaxf(fabsf(out[0]), fabsf(out[1])), fmaxf(fabsf(out[2]), fabsf(out[3])));
 #pragma unroll
   for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const float d = __fdiv_rn(amax, 127.0f);
   uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) w |= (uint32_t)((amax == 0.0f ? 0 : (int)roundf(__fdiv_rn(y[i], d))) & 0xFF) << (8 * i);
+  for (int i = 0; i < 4; i++) w |= (uint32_t)((amax == 0.0f ? 0 : (int)roundf(__fdiv_rn(out[i], d))) & 0xFF) << (8 * i);
   *(uint32_t*)(p.xq + row * AD + 4 * c) = w;
   if ((c & 7) == 0) p.xd[(row * AD + 4 * c) / 32] = __half2float(__float2half_rn(d));
 }
 
-// Rounds a workspace of `floats` down to the splits that it holds of `rows` rows.
-int64_t splits_that_fit(size_t floats, int64_t rows) { return (int64_t)(floats / ((size_t)rows * (AD + 2))); }
-
-// Partials of `rows` rows in *nsplit splits: in the prefill workspace, whose size is fixed (fewer splits where it holds no
-// more), or, for a batch, in the paged workspace.
-int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t nsplit, const char* who) {
-  float* part;
-  if (p.c.page_table) {
-    if (int rc = paged_ws(ctx, (size_t)rows * nsplit * (AD + 2), &part)) return rc;
-  } else {
-    size_t cap;
-    if (int rc = prefill_ws(ctx, &part, &cap)) return rc;
-    const int64_t fit = splits_that_fit(cap, rows);
-    if (fit < 1)
-      return fail(Q27B_UNSUPPORTED, std::string(who) + ": the prefill workspace (" + std::to_string(cap * sizeof(float)) +
-                                        " bytes) is too small for the partials of this call (" +
-                                        std::to_string((size_t)rows * (AD + 2) * sizeof(float)) + " bytes)");
-    nsplit = std::min(nsplit, fit);
-  }
-  p.nsplit = (int)nsplit;
-  p.part_o = part;
-  p.part_ml = (float2*)(part + (size_t)rows * nsplit * AD);
+int launch_rows_merge(const RowsParams& p, int64_t rows, int n_sm, cudaStream_t s) {
+  if (rows >= 8 * (int64_t)n_sm) Q27B_CK(launch_step(rows_merge_kernel<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p, rows));
+  else Q27B_CK(launch_step(rows_merge_kernel<4>, dim3((unsigned)rows), dim3(256), 0, s, p, rows));
   return Q27B_OK;
 }
+
+// Room for the partials of `rows` rows (and `more` floats behind them): in the prefill workspace, whose size is fixed, or, for a
+// batch, in the paged workspace. *fit: as many of `rows` as there is room for (a batch: all).
+int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t more, int64_t* fit, float** part) {
+  const size_t floats = (size_t)rows * (AD + 2) + (size_t)more;
+  *fit = rows;
+  if (p.c.page_table) return paged_ws(ctx, floats, part);
+  size_t cap;
+  if (int rc = prefill_ws(ctx, part, &cap)) return rc;
+  if (cap < floats) *fit = cap < (size_t)more ? 0 : (int64_t)((cap - (size_t)more) / (AD + 2));
+  return Q27B_OK;
+}
+int no_room(const char* who) { return fail(Q27B_UNSUPPORTED, std::string(who) + ": the prefill workspace is too small for the partials of this call"); }
 
 // How lists of k blocks are cut into chunks, a CTA each: the plan of the least time in a model of the launch (us). A round of CTAs
 // costs C0 and so much a block: an SM to itself for a CTA of two tile groups 0.71 (q8_0) or 1.1 (f16), for one of one group
@@ -157,10 +185,15 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   const BlocksPlan plan = plan_blocks(lists, p.k, ctx->n_sm, c.q8);
   const int nch = plan.nch;
   const WsGroups groups = plan.groups;
-  if (int rc = place_partials(ctx, p, rows, nch, who)) return rc;
-  const int chunk = (p.k + p.nsplit - 1) / p.nsplit;
-  if (chunk > SEL_CHUNK) return fail(Q27B_UNSUPPORTED, std::string(who) + ": the workspace is too small for the partials of this call");
+  float* part;
+  int64_t fit;
+  if (int rc = place_partials(ctx, p, rows * nch, 0, &fit, &part)) return rc;
+  if (fit < rows) return no_room(who);
+  const int chunk = (p.k + (int)(fit / rows) - 1) / (int)(fit / rows);
+  if (chunk > SEL_CHUNK) return no_room(who);
   p.nsplit = (p.k + chunk - 1) / chunk;
+  p.part_o = part;
+  p.part_ml = (float2*)(part + rows * p.nsplit * AD);
   DecodeParams d = {};
   d.qn = p.qn; d.pos0 = c.pos0; d.status = c.status; d.T = 1; d.nqh = c.nkvh * GQA; d.nkvh = c.nkvh; d.n_ctx = c.n_ctx;
   d.nch = p.nsplit; d.kq_scale = p.kq_scale; d.n_local = -1; d.page_table = c.page_table; d.seq_len = c.seq_len;
@@ -177,27 +210,29 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
     if (int rc = cached_tmap_2d(&vv, p.vcache, cache, 2 * AD, 2 * AD, 128, BLK, true)) return rc;
     if (int rc = launch_blocks_f16(&kv, &vv, d, c.B * c.T, s)) return rc;
   }
-  Q27B_CK(launch_step(rows_merge_kernel, dim3((unsigned)rows), dim3(256), 0, s, p));
-  return Q27B_OK;
+  return launch_rows_merge(p, rows, ctx->n_sm, s);
 }
 
-// One sequence: a CTA per SM, the positions of every row tile in equal shares. A batch: shares of equal length, so that the
-// sequences' CTAs come to about four rounds of the SMs if all are of the largest length.
 int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
-  const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, ctas = (int64_t)p.c.B * p.c.nkvh * tree_row_tiles(p.c.T);
-  const int64_t tiles = tree_tiles(p.c.n_ctx);
-  int64_t ns;
-  if (p.c.page_table) {
-    const int64_t share = std::min<int64_t>(TREE_MAX_SHARE, std::max<int64_t>(8, ctas * tiles / (4 * ctx->n_sm)));
-    p.share = (int)share;
-    ns = (tiles + share - 1) / share;
-  } else {
-    ns = std::max<int64_t>(1, std::min(tiles, ctx->n_sm / ctas));
+  const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, units = (int64_t)p.c.B * p.c.nkvh * tree_row_tiles(p.c.T);
+  const bool paged = p.c.page_table != nullptr;
+  const int64_t head = paged ? (2 * (p.c.B + 1) + 3) / 4 * 4 : 0;  // the plan, in floats
+  // One sequence: a CTA per SM (its shared and tensor memory take one), the same number for every unit.
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ctx->n_sm / units, tree_tiles(p.c.n_ctx))), fit;
+  int64_t slots = paged ? tree_grid(units, ctx->n_sm) : units * parts;
+  float* part;
+  if (int rc = place_partials(ctx, p, slots * TREE_ROWS, head, &fit, &part)) return rc;
+  if (fit < slots * TREE_ROWS) {
+    parts = fit / (units * TREE_ROWS);
+    if (parts < 1) return no_room(who);
+    slots = units * parts;
   }
-  if (int rc = place_partials(ctx, p, rows, ns, who)) return rc;
-  if (int rc = launch_tree(p, s)) return rc;
-  Q27B_CK(launch_step(rows_merge_kernel, dim3((unsigned)rows), dim3(256), 0, s, p));
-  return Q27B_OK;
+  p.nsplit = (int)parts;
+  p.plan = (int64_t*)part;
+  p.part_o = part + head;
+  p.part_ml = (float2*)(p.part_o + slots * TREE_ROWS * AD);
+  if (int rc = launch_tree(p, ctx->n_sm, s)) return rc;
+  return launch_rows_merge(p, rows, ctx->n_sm, s);
 }
 
 }  // namespace
@@ -251,6 +286,8 @@ int q27b_attn_decode_tree_paged(const float* qn, const float* qg, const void* kp
   RowsParams p = {};
   p.c = paged_ref(ctx, page_table, seq_len, B, T, nkvh, n_pages, max_pages);
   p.c.n_ctx = max_seq_len;  // a longer sequence is cut there
+  if (tree_tiles(max_seq_len) > TREE_MAX_TILES)
+    return fail(Q27B_UNSUPPORTED, "attn_decode_tree_paged: sequences of more than " + std::to_string(TREE_MAX_TILES * BLK) + " positions");
   p.qn = qn; p.qg = qg; p.kcache = kpool; p.vcache = vpool; p.o = o; p.xq = xq; p.xd = xd; p.mask = mask; p.kq_scale = kq_scale;
   return run_tree(ctx, p, "attn_decode_tree_paged", (cudaStream_t)stream);
 }

@@ -5,8 +5,10 @@
 // when the true one has outgrown it by TAU. Q kq_scale, K and V (q8_0: value times scale) and P are rounded to f16, the
 // operand type; m, the row sums and O are f32.
 //
-// One CTA takes 128 of the 6 T (draft, head) rows of a KV head over one share of the position tiles, and writes its m, l
-// and O as a partial: the prefix belongs to all rows, so up to 21 drafts cost one pass over the cache. A tile that reaches into
+// A unit is 128 of the 6 T (draft, head) rows of a KV head of a sequence: the prefix belongs to all rows, so up to 21 drafts cost
+// one pass over the cache. One CTA takes one part of a unit's position tiles and writes m, l and O as a partial. One sequence: a
+// CTA per SM, the same number for every unit. A batch: every CTA adds up the lengths, from which the length of a part follows
+// (tree_share), and finds its own part. A tile that reaches into
 // the drafted rows gets a 64-bit word of visible columns per row: the row's mask, shifted to the tile.
 // Weights of columns that a row does not see are 0, and so that 0 times what lies there is 0, V rows that no row
 // may see (past the sequence, on a page that does not exist) are cleared on the way to the tensor core, and drafted V
@@ -14,7 +16,7 @@
 //
 // Warps 0-7 softmax (two threads a row, 32 columns of a tile each), warp 8 issues the Q K^T MMAs, warp 9 the P V MMAs. f16
 // cache: warp 10 brings the tiles by TMA as the tensor core reads them. q8_0 cache: warps 10-13 turn K and 14-17 V into f16
-// operands, from registers that they load straight from the cache, a tile ahead (and three tiles ahead into L2): through shared
+// operands, from registers that they load straight from the cache, a tile ahead: through shared
 // memory, which 64 KB of operands a tile written and read again keep busy already, the int8 tile would cost another 68 KB.
 // TMEM: columns 0-255 O (f32), 256-383 two S buffers of 64 columns (f32), 384-511 the Q tile. (P over the scores it was made of
 // saves a store and a load of shared memory, but the next Q K^T then waits for P V: 102 us behind 150,000.)
@@ -41,8 +43,9 @@ constexpr int OFF_P = OFF_V + NV * KV_BYTES;
 constexpr int OFF_XCH = OFF_P + NP * P_BYTES;                  // [tile parity][NWG][128] f32
 constexpr int OFF_BAR = OFF_XCH + 2 * NWG * QT * 4;
 constexpr int OFF_BAD = OFF_BAR + NBAR * 8;               // [16 chunks of 16 dims][2 words]: drafts whose V chunk is not finite
-constexpr int OFF_SKIP = OFF_BAD + 16 * 8;                // [TREE_MAX_SHARE / 32] words: tiles on pages that do not exist
-constexpr int OFF_MISC = OFF_SKIP + TREE_MAX_SHARE / 8;
+constexpr int OFF_SKIP = OFF_BAD + 16 * 8;                // [TREE_MAX_TILES / 32] words: tiles on pages that do not exist
+constexpr int OFF_SCAN = OFF_SKIP + TREE_MAX_TILES / 8;   // [32] 64-bit sums
+constexpr int OFF_MISC = OFF_SCAN + 32 * 8;
 constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
 static_assert(SMEM_BYTES <= 232448, "shared memory budget of one CTA");
 constexpr int threads(bool q8) { return (NSW + 2 + (q8 ? 2 * N_CONV_WARPS : 1)) * 32; }
@@ -51,6 +54,13 @@ constexpr uint32_t TM_O = 0, TM_S = 256, TM_Q = 384;  // O f32 256 columns, S 2 
 constexpr uint32_t IDESC_QK = umma_idesc(1, 0, 0, 0, 0, QT, PT);   // f32 += f16 * f16, both K-major, M128 N64
 constexpr uint32_t IDESC_PV = umma_idesc(1, 0, 0, 0, 1, QT, AD);   // B (V) MN-major, M128 N256
 
+// One lane of a converged warp, the same one every time; in code that the compiler knows to be one lane's, the operands of
+// an MMA stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
 // the threads of a query row sit in warp q of every softmax warpgroup
 __device__ __forceinline__ void row_sync(int q) { asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "n"(32 * NWG) : "memory"); }
 __device__ __forceinline__ bool not_finite(uint32_t h2) { return (h2 & 0x7C00u) == 0x7C00u || (h2 & 0x7C000000u) == 0x7C000000u; }
@@ -83,7 +93,7 @@ __device__ __forceinline__ uint4 load16(const uint8_t* p) {
 
 template <bool Q8, bool PAGED>
 __global__ void __launch_bounds__(threads(Q8), 1)
-tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const RowsParams p) {
+tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const RowsParams p, int n_sm) {
   constexpr int THREADS = threads(Q8);
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -94,13 +104,89 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   uint32_t* tmem_slot = (uint32_t*)(sgen + OFF_MISC);
   volatile int* abort_flag = (volatile int*)(sgen + OFF_MISC + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int T = p.c.T, nkvh = p.c.nkvh, nqh = nkvh * GQA, z = blockIdx.x, kh = blockIdx.y % nkvh, row0 = (blockIdx.y / nkvh) * QT,
-            b = blockIdx.z;
-  // Softmax warps q, q + 4 have rows 32 q ..; those past the last row have nothing to do (what the tensor core makes of their rows
-  // of Q and P reaches no other row).
-  const int rows_here = T * GQA - row0, n_active = NWG * min(4, (rows_here + 31) / 32);
+  const int T = p.c.T, nkvh = p.c.nkvh, nqh = nkvh * GQA, units = nkvh * tree_row_tiles(T);  // units of a sequence
+  int64_t* scan = (int64_t*)(sgen + OFF_SCAN);
 
   // What needs no memory of the call runs while the previous kernel of the stream drains.
+  if (tid == 0) {
+    *abort_flag = 0;
+    if (!Q8) {
+      tma_prefetch_desc(&tm_k);
+      tma_prefetch_desc(&tm_v);
+    }
+  }
+  pdl_wait();
+  pdl_trigger();
+  // The part of this CTA: tiles it0 .. it0 + nt - 1 of unit y (a row tile of a KV head) of sequence b
+  auto end_of = [&](int b) { return min(first_pos(p.c, b) + T, p.c.n_ctx); };
+  int b = 0, y = 0, it0 = 0, nt = 0;
+  if (!PAGED) {
+    const int ntot = tree_tiles(end_of(0)), parts = min(p.nsplit, ntot), z = blockIdx.x % p.nsplit;
+    y = blockIdx.x / p.nsplit;
+    if (z < parts) it0 = (int)((int64_t)ntot * z / parts), nt = (int)((int64_t)ntot * (z + 1) / parts) - it0;
+  } else {  // every thread looks at some sequences: the tiles of all of them, then their parts
+    const int per = (p.c.B + THREADS - 1) / THREADS, b0 = min(p.c.B, tid * per), b1 = min(p.c.B, b0 + per);
+    int64_t mine = 0, all = 0;
+    auto sum = [&](int64_t v) {  // -> the sum before this thread's; `all`: of all
+      int64_t x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t t = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += t;
+      }
+      if (lane == 31) scan[warp] = x;
+      __syncthreads();
+      int64_t before = 0;
+      all = 0;
+      for (int w = 0; w < THREADS / 32; w++) {
+        if (w < warp) before += scan[w];
+        all += scan[w];
+      }
+      __syncthreads();
+      return before + x - v;
+    };
+    for (int i = b0; i < b1; i++) {
+      const int n = tree_tiles(end_of(i));
+      mine += n ? ((int64_t)1 << 40) + n : 0;  // sequences that are not empty, and their tiles
+    }
+    sum(mine);
+    const int share = tree_share((all & (((int64_t)1 << 40) - 1)) * units, (all >> 40) * units, n_sm);
+    mine = 0;
+    for (int i = b0; i < b1; i++) mine += tree_parts(tree_tiles(end_of(i)), share);
+    int64_t at = sum(mine);
+    if (tid == 0) scan[0] = -1;
+    __syncthreads();
+    for (int i = b0; i < b1; i++) {
+      const int n = tree_parts(tree_tiles(end_of(i)), share);
+      if (blockIdx.x == 0) p.plan[1 + i] = at;
+      if (at * units <= blockIdx.x && blockIdx.x < (at + n) * units) scan[0] = i, scan[1] = at;
+      at += n;
+    }
+    if (blockIdx.x == 0 && tid == 0) p.plan[0] = share;
+    __syncthreads();
+    b = (int)scan[0];
+    if (b >= 0) {
+      const int ntot = tree_tiles(end_of(b)), parts = tree_parts(ntot, share), k = (int)(blockIdx.x - scan[1] * units), z = k % parts;
+      y = k / parts;
+      it0 = (int)((int64_t)ntot * z / parts), nt = (int)((int64_t)ntot * (z + 1) / parts) - it0;
+    }
+  }
+  if (nt > 0 && warp == 0) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (nt <= 0) return;  // the merge knows which parts there are
+  const uint32_t tmem = *tmem_slot;
+  const int first = first_pos(p.c, b);  // of the drafts
+  const int n_end = end_of(b), zone = min(first, n_end);  // rows from `zone` on are not for everybody
+  const int kh = y % nkvh, row0 = y / nkvh * QT;
+  const int64_t slot0 = (int64_t)blockIdx.x * QT;  // its rows among the partials
+  // Softmax warps q, q + 4 have rows 32 q ..; those past the last row have nothing to do (what the tensor core makes of their rows
+  // of Q and P reaches no other row).
+  const int n_active = NWG * min(4, (T * GQA - row0 + 31) / 32);
   if (tid == 0) {
     mbar_init(&bar[B_QFULL], n_active);
     for (int s = 0; s < 3; s++) {
@@ -118,35 +204,16 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       mbar_init(&bar[B_PVDONE + s], 1);
     }
     mbar_init(&bar[B_ODONE], 1);
-    *abort_flag = 0;
     mbar_fence_init();
-    if (!Q8) {
-      tma_prefetch_desc(&tm_k);
-      tma_prefetch_desc(&tm_v);
-    }
   }
   if (tid < 32) bad[tid] = 0;
-  if (PAGED && tid >= 32 && tid < 32 + TREE_MAX_SHARE / 32) skip[tid - 32] = 0;
-  pdl_wait();
-  pdl_trigger();
-  const int first = first_pos(p.c, b);  // of the drafts
-  const int n_end = min(first + T, p.c.n_ctx), zone = min(first, n_end);  // rows from `zone` on are not for everybody
-  const int ntot = tree_tiles(n_end), share = tree_share(p, ntot);
-  const int it0 = min(ntot, z * share), nt = min(ntot, it0 + share) - it0;
-  if (nt <= 0) return;  // the merge knows which shares hold tiles
-  if (warp == MMA_WARP) {
-    tmem_alloc(tmem_slot, TMEM_COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  if (PAGED) {  // the pages of this share: what lies on one that is none is not visible
+  if (PAGED) {  // the pages of this part: what lies on one that is none is not visible
+    for (int j = tid; j < (nt + 31) / 32; j += THREADS) skip[j] = 0;
+    __syncthreads();
     for (int j = tid; j < nt; j += THREADS)
       if (cache_row(p.c, b, kh, (it0 + j) * PT) < 0) atomicOr(&skip[j >> 5], 1u << (j & 31));
-    __syncthreads();
   }
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  __syncthreads();
   auto skipped = [&](int j) { return PAGED && ((((volatile uint32_t*)skip)[j >> 5] >> (j & 31)) & 1); };
 
   if (warp < NSW && (warp & 3) >= n_active / NWG) {
@@ -309,7 +376,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     row_sync(q);
 #pragma unroll
     for (int o = 1; o < NWG; o++) l += xch[((nt & 1) * NWG + ((wg + o) % NWG)) * QT + r];
-    if (wg == 0 && t < T) p.part_ml[out_row(row0 + r) * p.nsplit + z] = make_float2(m_ref, l);
+    if (wg == 0 && t < T) p.part_ml[slot0 + r] = make_float2(m_ref, l);
     mbar_wait(&bar[B_ODONE], 0, abort_flag, p.c.status);
     tc_fence_after();
     // 32 columns at a time through shared memory (the K buffers are free now): TMEM gives a thread a row, and a row per
@@ -337,51 +404,56 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       for (int i = 0; i < 8; i++) {
         const int rr = 4 * i + (lane >> 3), gr = row0 + q * 32 + rr;
         if (gr >= T * GQA) continue;
-        *(float4*)(p.part_o + (out_row(gr) * p.nsplit + z) * AD + d0 + 4 * (lane & 7)) = *(const float4*)(stage + swz128(rr, lane & 7));
+        *(float4*)(p.part_o + (slot0 + q * 32 + rr) * AD + d0 + 4 * (lane & 7)) = *(const float4*)(stage + swz128(rr, lane & 7));
       }
       __syncwarp();
     }
     tc_fence_before();
   } else if (warp == MMA_WARP) {
     // ================================================================ Q K^T issuer
-    if (lane == 0) {
-      mbar_wait(&bar[B_QFULL], 0, abort_flag, p.c.status);
-      tc_fence_after();
+    mbar_wait(&bar[B_QFULL], 0, abort_flag, p.c.status);
+    const bool issuer = elect_one();
+    const uint64_t desc = umma_desc_sw128(sbase + OFF_K, 16, 1024);
+    int st = 0, ph = 0;  // K buffer and its phase
 #pragma unroll 1
-      for (int j = 0; j < nt; j++) {
-        const int ss = j & 1, sph = (j >> 1) & 1;                         // S buffer
-        const int st = j % NK, ph = (j / NK) & 1;                         // K buffer
-        mbar_wait(&bar[B_KFULL + st], ph, abort_flag, p.c.status);
-        mbar_wait(&bar[B_SEMPTY + ss], sph ^ 1, abort_flag, p.c.status);
-        tc_fence_after();
+    for (int j = 0; j < nt; j++) {
+      const int ss = j & 1, sph = (j >> 1) & 1;                         // S buffer
+      mbar_wait(&bar[B_KFULL + st], ph, abort_flag, p.c.status);
+      mbar_wait(&bar[B_SEMPTY + ss], sph ^ 1, abort_flag, p.c.status);
+      tc_fence_after();
+      if (issuer) {
 #pragma unroll
-        for (int kk = 0; kk < AD / 16; kk++) {
-          const uint64_t db = umma_desc_sw128(sbase + OFF_K + st * KV_BYTES + (kk >> 2) * SEGK + (kk & 3) * 32, 16, 1024);
-          tc_mma_f16_ts(tmem + TM_S + ss * PT, tmem + TM_Q + kk * 8, db, IDESC_QK, kk > 0 ? 1u : 0u);
-        }
+        for (int kk = 0; kk < AD / 16; kk++)  // (addresses of a descriptor are in units of 16 bytes)
+          tc_mma_f16_ts(tmem + TM_S + ss * PT, tmem + TM_Q + kk * 8, desc + (uint64_t)(st * (KV_BYTES / 16) + ((kk >> 2) * SEGK + (kk & 3) * 32) / 16),
+                        IDESC_QK, kk > 0 ? 1u : 0u);
         tc_commit(&bar[B_SFULL + ss]);
         tc_commit(&bar[B_KEMPTY + st]);
       }
+      __syncwarp();
+      if (++st == NK) st = 0, ph ^= 1;
     }
   } else if (warp == PV_WARP) {
     // ================================================================ P V issuer
-    if (lane == 0) {
+    const bool issuer = elect_one();
+    const uint64_t desc_p = umma_desc_sw128(sbase + OFF_P, 16, 1024), desc_v = umma_desc_sw128(sbase + OFF_V, SEGK, 1024);
+    int st = 0, ph = 0;  // V buffer and its phase
 #pragma unroll 1
-      for (int j = 0; j < nt; j++) {
-        const int st = j % NV, ph = (j / NV) & 1, pb = j & 1;
-        mbar_wait(&bar[B_PFULL + pb], (j >> 1) & 1, abort_flag, p.c.status);
-        mbar_wait(&bar[B_VFULL + st], ph, abort_flag, p.c.status);
-        tc_fence_after();
+    for (int j = 0; j < nt; j++) {
+      const int pb = j & 1;
+      mbar_wait(&bar[B_PFULL + pb], (j >> 1) & 1, abort_flag, p.c.status);
+      mbar_wait(&bar[B_VFULL + st], ph, abort_flag, p.c.status);
+      tc_fence_after();
+      if (issuer) {
 #pragma unroll
-        for (int kk = 0; kk < PT / 16; kk++) {
-          const uint64_t db = umma_desc_sw128(sbase + OFF_V + st * KV_BYTES + kk * 2048, SEGK, 1024);
-          const uint64_t da = umma_desc_sw128(sbase + OFF_P + pb * P_BYTES + kk * 32, 16, 1024);
-          tc_mma_f16(tmem + TM_O, da, db, IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
-        }
+        for (int kk = 0; kk < PT / 16; kk++)
+          tc_mma_f16(tmem + TM_O, desc_p + (uint64_t)(pb * (P_BYTES / 16) + kk * 2), desc_v + (uint64_t)(st * (KV_BYTES / 16) + kk * 128),
+                     IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
         tc_commit(&bar[B_PVDONE + pb]);
         tc_commit(&bar[B_VEMPTY + st]);
+        if (j == nt - 1) tc_commit(&bar[B_ODONE]);
       }
-      tc_commit(&bar[B_ODONE]);
+      __syncwarp();
+      if (++st == NV) st = 0, ph ^= 1;
     }
   } else if constexpr (!Q8) {
     // ================================================================ TMA producer (f16 cache)
@@ -434,13 +506,6 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       x[k] = load16(src + r * AD);
       d[k] = whole || 8 * k < there ? *(const uint16_t*)(ssrc + r * 16) : 0;
     };
-    auto to_l2 = [&](int j) {
-      if (ct != 0 || j >= nt || tile_rows(j) <= 0) return;
-      const int64_t row = tile_row(j);
-      const uint32_t rows = (uint32_t)tile_rows(j);
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(vals + row * AD), "r"(rows * AD) : "memory");
-      asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(scales + row * 16), "r"(rows * 16) : "memory");
-    };
     // Item k of the tile in registers into the f16 buffer, and the same item of the next tile fetched in its place.
     auto convert = [&](int k, uint8_t* dst, bool more, bool whole, int drafted) {
       const __half2 dd = u32_as_h2(__byte_perm(d[k], d[k], 0x1010));
@@ -468,14 +533,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     aim(0);
 #pragma unroll
     for (int k = 0; k < 8; k++) fetch(k, false);
-    to_l2(1);
-    to_l2(2);
     const int nbuf = is_v ? NV : NK;
     int fb = 0, ph = 1;
 #pragma unroll 1
     for (int j = 0; j < nt; j++) {
       const int p_tile = (it0 + j) * PT;
-      to_l2(j + 3);
       const bool more = j + 1 < nt;
       if (more) aim(j + 1);
       mbar_wait(&bar[b_empty + fb], ph, abort_flag, p.c.status);  // the MMAs of the tile before it have read the buffer
@@ -500,7 +562,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   drain_after_abort(abort_flag);
   tc_fence_before();
   __syncthreads();
-  if (warp == MMA_WARP) {
+  if (warp == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
@@ -514,7 +576,7 @@ int tree_attr() {
 
 }  // namespace
 
-int launch_tree(const RowsParams& p, cudaStream_t s) {
+int launch_tree(const RowsParams& p, int n_sm, cudaStream_t s) {
   static bool attr[64] = {};
   static std::mutex attr_mu;
   int dev;
@@ -528,17 +590,18 @@ int launch_tree(const RowsParams& p, cudaStream_t s) {
       attr[dev] = true;
     }
   }
-  const dim3 grid(p.nsplit, p.c.nkvh * tree_row_tiles(p.c.T), p.c.B);
+  const int64_t units = (int64_t)p.c.B * p.c.nkvh * tree_row_tiles(p.c.T);
+  const dim3 grid((unsigned)(p.c.page_table ? tree_grid(units, n_sm) : units * p.nsplit));
   CUtensorMap tk = {}, tv = {};  // f16 only
   if (p.c.page_table) {
-    Q27B_CK(launch_step(tree_kernel<true, true>, grid, dim3(threads(true)), SMEM_BYTES, s, tk, tv, p));
+    Q27B_CK(launch_step(tree_kernel<true, true>, grid, dim3(threads(true)), SMEM_BYTES, s, tk, tv, p, n_sm));
   } else if (p.c.q8) {
-    Q27B_CK(launch_step(tree_kernel<true, false>, grid, dim3(threads(true)), SMEM_BYTES, s, tk, tv, p));
+    Q27B_CK(launch_step(tree_kernel<true, false>, grid, dim3(threads(true)), SMEM_BYTES, s, tk, tv, p, n_sm));
   } else {
     const uint64_t rows = cache_rows(p.c);
     if (int rc = cached_tmap_2d(&tk, p.kcache, rows, 2 * AD, 2 * AD, 128, PT, true)) return rc;
     if (int rc = cached_tmap_2d(&tv, p.vcache, rows, 2 * AD, 2 * AD, 128, PT, true)) return rc;
-    Q27B_CK(launch_step(tree_kernel<false, false>, grid, dim3(threads(false)), SMEM_BYTES, s, tk, tv, p));
+    Q27B_CK(launch_step(tree_kernel<false, false>, grid, dim3(threads(false)), SMEM_BYTES, s, tk, tv, p, n_sm));
   }
   return Q27B_OK;
 }
