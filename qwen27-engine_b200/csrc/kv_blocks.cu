@@ -189,8 +189,8 @@ __device__ __forceinline__ int blocks_of(const CacheRef& c, int b, int t) {
 // A warp scores 16 blocks of a (KV head, sequence) for all its tokens with m16n8k16 MMAs: the bounds are the A operand as they
 // lie in memory (a lane's 16 bytes are two k-steps; the order of the dims is free), all of them in registers at once, the
 // query heads are six of the eight columns of B. q times a power of two, so that its largest value is below 2^10, is the sum
-// of two f16 values, off by at most 2^-22 of itself or 2^-25. Three accumulators: q+ hi and q- lo with the larger parts, 16 MMAs
-// each, and both with the smaller parts. With A = sum |q| max(|lo|, |hi|) (a fourth one, of |q| + 2^-6), and 17 addends of
+// of two f16 values, off by at most 2^-22 of itself or 2^-25. Four accumulators: q+ hi and q- lo, with the larger parts and with
+// the smaller ones, 16 MMAs each. With A = sum |q| max(|lo|, |hi|) (a fifth one, of |q| + 2^-6), and 17 addends of
 // an MMA each cut at 2^-23 of the largest, the error is below 16 * 18 * 2^-23 A + 2^-22 A < 2^-14.7 A; 2^-14 A is what is
 // passed on. Bound by reading the bounds once they fill the SMs.
 constexpr int SCORE_WARPS = 4, SCORE_GROUP = 16 * SCORE_WARPS, Q_STRIDE = 2 * AD + 64;  // bytes between staged query rows: 16-byte reads without conflicts
@@ -261,10 +261,17 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const Select
 #pragma unroll 1
   for (int group = blockIdx.x; group < ngroups; group += gridDim.x) {
     if (group != (int)blockIdx.x) load(group);
+    const int ahead = (group + gridDim.x) * SCORE_GROUP + 16 * warp + (lane >> 1);  // the next group's bounds into L2, half a block a lane
+    if (ahead < nb) {
+      const int64_t at = bounds_index(p.c, b, kh, ahead);
+      if (at >= 0)
+#pragma unroll
+        for (int i = 0; i < 4; i++) prefetch_l2(p.bounds + at * 2 * AD + (lane & 1) * AD + 64 * i);
+    }
 #pragma unroll 1
     for (int t = 0; t < T; t++) {
       const uint8_t* qt = sq + t * Q_TOKEN + g * Q_STRIDE + 16 * tg;
-      float sp[4] = {}, sm[4] = {}, sl[4] = {}, sa[4] = {};
+      float sp[4] = {}, sm[4] = {}, sl[4] = {}, sn[4] = {}, sa[4] = {};
 #pragma unroll
       for (int j = 0; j < 8; j++) {
         uint4 q[Q_PARTS];
@@ -276,9 +283,9 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const Select
         mma16816(sl, h0.x, h1.x, h0.y, h1.y, q[QP_LO].x, q[QP_LO].y);
         mma16816(sp, h0.z, h1.z, h0.w, h1.w, q[QP_HI].z, q[QP_HI].w);
         mma16816(sm, l0.z, l1.z, l0.w, l1.w, q[QM_HI].z, q[QM_HI].w);
-        mma16816(sl, l0.x, l1.x, l0.y, l1.y, q[QM_LO].x, q[QM_LO].y);
+        mma16816(sn, l0.x, l1.x, l0.y, l1.y, q[QM_LO].x, q[QM_LO].y);
         mma16816(sl, h0.z, h1.z, h0.w, h1.w, q[QP_LO].z, q[QP_LO].w);
-        mma16816(sl, l0.z, l1.z, l0.w, l1.w, q[QM_LO].z, q[QM_LO].w);
+        mma16816(sn, l0.z, l1.z, l0.w, l1.w, q[QM_LO].z, q[QM_LO].w);
         const auto widest = [](uint32_t x, uint32_t y) { return h2_as_u32(__hmax2_nan(__habs2(u32_as_h2(x)), __habs2(u32_as_h2(y)))); };
         mma16816(sa, widest(l0.x, h0.x), widest(l1.x, h1.x), widest(l0.y, h0.y), widest(l1.y, h1.y), q[QABS].x, q[QABS].y);
         mma16816(sa, widest(l0.z, h0.z), widest(l1.z, h1.z), widest(l0.w, h0.w), widest(l1.w, h1.w), q[QABS].z, q[QABS].w);
@@ -291,7 +298,7 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const Select
         if (tg < 3) {
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const float u = unit[t][2 * tg + i], v = (sp[2 * e + i] + sm[2 * e + i] + sl[2 * e + i]) * u, a = sa[2 * e + i] * u * 6.2e-5f;
+            const float u = unit[t][2 * tg + i], v = (sp[2 * e + i] + sm[2 * e + i] + (sl[2 * e + i] + sn[2 * e + i])) * u, a = sa[2 * e + i] * u * 6.2e-5f;
             odd |= !(fabsf(v) <= 3e38f) || !(a <= 3e38f);
             best = fmaxf(best, v);
             err = fmaxf(err, a);
@@ -320,6 +327,7 @@ struct SelShared {
   uint64_t key_red[2][SEL_WARPS];
   float red[SEL_WARPS];
   int bin, need, inside, n_in, n_open;
+  alignas(16) float q[GQA][AD];
   uint32_t in[SEL_MAX_BLOCKS / 32], edge[SEL_MAX_BLOCKS / 32];  // a bit per block: is chosen; is chosen while there is room
 };
 
@@ -415,7 +423,7 @@ __device__ K nth_largest(F key, int n, int want, int few, SelShared& sh, K* mask
 // out; the scores of the blocks with s <= t1 are at most t1 + E, and fewer than want have a larger s, so a block of s - e > t1 + E
 // is in. The blocks between are scored again in 64 bits, a warp each, and the best of them fill up the list; of equal ones the
 // lower. Where something is not finite, or everything alike, these are all blocks. Bound by the latency of a dozen barriers.
-__global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectParams p) {
+__global__ void __launch_bounds__(SEL_THREADS, 2) select_kernel(const SelectParams p) {
   extern __shared__ uint64_t dyn[];  // [max_blocks] (score, error), then the 64-bit keys of the open blocks; then their numbers
   __shared__ SelShared sh;
   pdl_trigger();
@@ -439,6 +447,10 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectParams 
   float E = 0.f, above = INFINITY, below = INFINITY;  // want = 0: nothing between the ends
   if (want > 0) {
     const float2* src = p.score + row * p.max_blocks + lo;
+    const float* qn = p.qn + (tok * nqh + kh * GQA) * AD;
+#pragma unroll
+    for (int i = 0; i < GQA * AD / SEL_THREADS; i++) (&sh.q[0][0])[tid + i * SEL_THREADS] = qn[tid + i * SEL_THREADS];
+#pragma unroll 4
     for (int i = tid; i < n; i += SEL_THREADS) {
       const float2 v = src[i];
       score[i] = v;
@@ -487,11 +499,6 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectParams 
     __syncthreads();
   } else {
     uint64_t* key = dyn;  // the scores to 15 bits are no longer used
-    float q[GQA][8];
-#pragma unroll
-    for (int g = 0; g < GQA; g++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) q[g][i] = p.qn[(tok * nqh + kh * GQA + g) * AD + 8 * lane + i];
     for (int c = warp; c < n_open; c += SEL_WARPS) {
       const int64_t idx = bounds_index(p.c, b, kh, open[c]);
       double s[GQA] = {};
@@ -499,12 +506,13 @@ __global__ void __launch_bounds__(SEL_THREADS) select_kernel(const SelectParams 
         const uint4 l4 = *(const uint4*)(p.bounds + idx * 2 * AD + 8 * lane), h4 = *(const uint4*)(p.bounds + idx * 2 * AD + AD + 8 * lane);
         const uint32_t lw[4] = {l4.x, l4.y, l4.z, l4.w}, hw[4] = {h4.x, h4.y, h4.z, h4.w};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float2 lf = __half22float2(u32_as_h2(lw[i >> 1])), hf = __half22float2(u32_as_h2(hw[i >> 1]));
+        for (int i = 0; i < 4; i++) {
+          const float2 lf = __half22float2(u32_as_h2(lw[i])), hf = __half22float2(u32_as_h2(hw[i]));
 #pragma unroll
           for (int g = 0; g < GQA; g++) {
-            const double x = q[g][i];
-            s[g] = fma(x, (double)(q[g][i] < 0.f ? (i & 1 ? lf.y : lf.x) : (i & 1 ? hf.y : hf.x)), s[g]);
+            const float2 x = *(const float2*)&sh.q[g][8 * lane + 2 * i];
+            s[g] = fma((double)x.x, (double)(x.x < 0.f ? lf.x : hf.x), s[g]);
+            s[g] = fma((double)x.y, (double)(x.y < 0.f ? lf.y : hf.y), s[g]);
           }
         }
       }
