@@ -325,7 +325,7 @@ struct SelShared {
   unsigned int hist[SEL_BINS];
   unsigned long long sums[SEL_WARPS];
   uint64_t key_red[2][SEL_WARPS];
-  float red[SEL_WARPS];
+  float red[3][SEL_WARPS];
   int bin, need, inside, n_in, n_open;
   alignas(16) float q[GQA][AD];
   uint32_t in[SEL_MAX_BLOCKS / 32], edge[SEL_MAX_BLOCKS / 32];  // a bit per block: is chosen; is chosen while there is room
@@ -361,13 +361,42 @@ __device__ __forceinline__ uint64_t order_key(double s) {
   return bits >> 63 ? ~bits : bits | 0x8000000000000000ull;
 }
 
+// The bin of the histogram (2,048 bins, filled before a barrier) in which the count from the top reaches `want`, all 512 threads:
+// how many of its entries belong to the want largest, and how many it has. Leaves the histogram at zero.
+__device__ __forceinline__ int find_bin(int want, SelShared& sh, int* need, int* inside) {
+  constexpr int PER = SEL_BINS / SEL_THREADS;
+  const int tid = threadIdx.x, top = SEL_BINS - 1 - PER * tid;  // thread i looks at the four bins from 2047 - 4 i down
+  unsigned int h[PER], mine = 0;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    mine += h[j] = sh.hist[top - j];
+    sh.hist[top - j] = 0;
+  }
+  int above = (int)block_scan(mine, sh.sums);
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    if (above < want && above + (int)h[j] >= want) {
+      sh.bin = top - j;
+      sh.need = want - above;
+      sh.inside = (int)h[j];
+    }
+    above += (int)h[j];
+  }
+  __syncthreads();
+  const int bin = sh.bin;
+  *need = sh.need;
+  *inside = sh.inside;
+  __syncthreads();
+  return bin;
+}
+
 // Where the want-th largest (1 <= want <= n) of key(0) .. key(n - 1) lies, all 512 threads: eleven bits at a time from the
 // highest bit in which keys differ, until at most `few` keys share its leading bits. Returns those bits; *mask_out which they
 // are, *need_out how many of the keys that share them belong to the want largest. hist is zero on entry and on return.
 template <typename K, typename F>
 __device__ K nth_largest(F key, int n, int want, int few, SelShared& sh, K* mask_out, int* need_out) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  constexpr int BITS = 8 * sizeof(K), PER = SEL_BINS / SEL_THREADS;
+  constexpr int BITS = 8 * sizeof(K);
   K mn = ~(K)0, mx = 0;
   for (int i = tid; i < n; i += SEL_THREADS) mn = min(mn, key(i)), mx = max(mx, key(i));
 #pragma unroll
@@ -388,30 +417,9 @@ __device__ K nth_largest(F key, int n, int want, int few, SelShared& sh, K* mask
       if ((x & mask) == prefix) atomicAdd(&sh.hist[(unsigned)(x >> shift) & (SEL_BINS - 1)], 1u);
     }
     __syncthreads();
-    // thread i looks at the four bins from 2047 - 4 i down
-    unsigned int h[PER], mine = 0;
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      mine += h[j] = sh.hist[SEL_BINS - 1 - (PER * tid + j)];
-      sh.hist[SEL_BINS - 1 - (PER * tid + j)] = 0;
-    }
-    int above = (int)block_scan(mine, sh.sums);
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-      if (above < need && above + (int)h[j] >= need) {
-        sh.bin = SEL_BINS - 1 - (PER * tid + j);
-        sh.need = need - above;
-        sh.inside = (int)h[j];
-      }
-      above += (int)h[j];
-    }
-    __syncthreads();
-    need = sh.need;
-    inside = sh.inside;
-    prefix |= (K)sh.bin << shift;
+    prefix |= (K)find_bin(need, sh, &need, &inside) << shift;
     mask |= (K)(SEL_BINS - 1) << shift;
     shift = max(0, shift - SEL_BITS);
-    __syncthreads();
   }
   *mask_out = mask;
   *need_out = need;
@@ -444,34 +452,63 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) select_kernel(const SelectPara
   const int words = (nb + 31) / 32;
   float2* score = (float2*)dyn;
   uint16_t* open = (uint16_t*)(dyn + p.max_blocks);
-  float E = 0.f, above = INFINITY, below = INFINITY;  // want = 0: nothing between the ends
+  float above = INFINITY, below = INFINITY;  // want = 0: nothing between the ends
   if (want > 0) {
     const float2* src = p.score + row * p.max_blocks + lo;
     const float* qn = p.qn + (tok * nqh + kh * GQA) * AD;
-#pragma unroll
-    for (int i = 0; i < GQA * AD / SEL_THREADS; i++) (&sh.q[0][0])[tid + i * SEL_THREADS] = qn[tid + i * SEL_THREADS];
+    float E = 0.f, mn = INFINITY, mx = -INFINITY;
 #pragma unroll 4
     for (int i = tid; i < n; i += SEL_THREADS) {
       const float2 v = src[i];
       score[i] = v;
       E = fmaxf(E, v.y);
+      mn = fminf(mn, v.x);
+      mx = fmaxf(mx, v.x);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) E = fmaxf(E, __shfl_xor_sync(0xffffffffu, E, o));
-    if (lane == 0) sh.red[warp] = E;
+    for (int i = 0; i < GQA * AD / SEL_THREADS; i++) (&sh.q[0][0])[tid + i * SEL_THREADS] = qn[tid + i * SEL_THREADS];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      E = fmaxf(E, __shfl_xor_sync(0xffffffffu, E, o));
+      mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    }
+    if (lane == 0) sh.red[0][warp] = E, sh.red[1][warp] = mn, sh.red[2][warp] = mx;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SEL_WARPS; w++) E = fmaxf(E, sh.red[w]);
+    for (int w = 0; w < SEL_WARPS; w++) {
+      E = fmaxf(E, sh.red[0][w]);
+      mn = fminf(mn, sh.red[1][w]);
+      mx = fmaxf(mx, sh.red[2][w]);
+    }
     if (E <= 3e38f) {
-      uint32_t mask;
-      int ignored;
-      const uint32_t lead = nth_largest<uint32_t>([&](int i) { return order_key(score[i].x); }, n, want, 16, sh, &mask, &ignored);
-      above = key_value(lead | ~mask) + E;
-      below = key_value(lead) - E;
+      // The scores in 2,048 steps from the smallest to the largest: the want-th largest lies in the step where the count from the top
+      // reaches want. The step's ends are moved out by more than the roundings of the arithmetic. Where the scores are too far
+      // apart or too close for that, or many lie in the step, by their bits.
+      const float width = mx - mn, scale = (float)SEL_BINS / width;
+      int inside = n;
+      const bool steps = width > 1e-30f && width < 1e30f;
+      if (steps) {
+        for (int i = tid; i < n; i += SEL_THREADS) atomicAdd(&sh.hist[min(SEL_BINS - 1, (int)((score[i].x - mn) * scale))], 1u);
+        __syncthreads();
+        int need;
+        const int bin = find_bin(want, sh, &need, &inside);
+        const float step = width / SEL_BINS, slack = 1e-6f * (fabsf(mn) + fabsf(mx));
+        above = mn + (float)(bin + 1) * step + slack + E;
+        below = mn + (float)bin * step - slack - E;
+      }
+      if (!steps || inside > 64) {
+        uint32_t mask;
+        int ignored;
+        const uint32_t lead = nth_largest<uint32_t>([&](int i) { return order_key(score[i].x); }, n, want, 16, sh, &mask, &ignored);
+        above = key_value(lead | ~mask) + E;
+        below = key_value(lead) - E;
+      }
     } else {
       below = -INFINITY;  // all are open (no s - e is above infinity)
     }
   }
+  int n_in = 0;
   for (int w = warp; w < words; w += SEL_WARPS) {
     const int blk = 32 * w + lane;
     bool in = blk < lo || (blk >= hi && blk < nb), maybe = false;
@@ -481,16 +518,16 @@ __global__ void __launch_bounds__(SEL_THREADS, 2) select_kernel(const SelectPara
       maybe = !in && !(v.x + v.y < below);
     }
     const uint32_t wi = __ballot_sync(0xffffffffu, in), wo = __ballot_sync(0xffffffffu, maybe);
-    int at = 0;
-    if (lane == 0) {
-      sh.in[w] = wi;
-      sh.edge[w] = 0;
-      if (wo) at = atomicAdd(&sh.n_open, __popc(wo));
-      if (wi) atomicAdd(&sh.n_in, __popc(wi));
+    n_in += __popc(wi);
+    if (lane == 0) sh.in[w] = wi, sh.edge[w] = 0;
+    if (wo) {
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sh.n_open, __popc(wo));
+      at = __shfl_sync(0xffffffffu, at, 0);
+      if (maybe) open[at + __popc(wo & ((1u << lane) - 1))] = (uint16_t)blk;
     }
-    at = __shfl_sync(0xffffffffu, at, 0);
-    if (maybe) open[at + __popc(wo & ((1u << lane) - 1))] = (uint16_t)blk;
   }
+  if (lane == 0 && n_in) atomicAdd(&sh.n_in, n_in);
   __syncthreads();
   const int n_open = sh.n_open, room = p.k - sh.n_in;  // 0 <= room <= n_open, by the above
   int need = 0;
