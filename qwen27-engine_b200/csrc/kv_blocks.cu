@@ -186,8 +186,8 @@ __device__ __forceinline__ int blocks_of(const CacheRef& c, int b, int t) {
   return last < 0 ? 0 : last / BLK + 1;
 }
 
-// A warp scores 16 blocks of a (KV head, sequence) for all its tokens with m16n8k16 MMAs: the bounds are the A operand as they
-// lie in memory (a lane's 16 bytes are two k-steps; the order of the dims is free), all of them in registers at once, the
+// A warp scores 16 blocks of a (KV head, sequence) for all its T tokens with m16n8k16 MMAs: the bounds are the A operand as they
+// lie in memory (a lane's 16 bytes are two k-steps; the order of the dims is free), all of them in registers at once (one token) or half, the
 // query heads are six of the eight columns of B. q times a power of two, so that its largest value is below 2^10, is the sum
 // of two f16 values, off by at most 2^-22 of itself or 2^-25. Four accumulators: q+ hi and q- lo, with the larger parts and with
 // the smaller ones, 16 MMAs each. With A = sum |q| max(|lo|, |hi|) (a fifth one, of |q| + 2^-6), and 17 addends of
@@ -197,36 +197,42 @@ constexpr int SCORE_WARPS = 4, SCORE_GROUP = 16 * SCORE_WARPS, Q_STRIDE = 2 * AD
 enum { QP_HI, QM_HI, QP_LO, QM_LO, QABS, Q_PARTS };
 constexpr int Q_TOKEN = Q_PARTS * 8 * Q_STRIDE;  // bytes of a staged token
 
-__global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const SelectParams p) {
+template <int T>
+__global__ void __launch_bounds__(32 * SCORE_WARPS, T == 2 ? 3 : 2) score_kernel(const SelectParams p) {
+  constexpr int TURNS = T == 1 ? 1 : 2, PER = 8 / TURNS;  // the dims in one or two turns of 32 PER
   extern __shared__ __align__(16) uint8_t sq[];  // [T][Q_PARTS][8 columns][Q_STRIDE]
-  __shared__ float unit[Q27B_MAX_T][8];          // 1 / scale of a head
+  __shared__ float unit[T][8];          // 1 / scale of a head
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tg = lane & 3;
-  const int kh = blockIdx.y, b = blockIdx.z, T = p.c.T, nqh = p.c.nkvh * GQA;
+  const int kh = blockIdx.y, b = blockIdx.z, nqh = p.c.nkvh * GQA;
   for (int i = tid; i < T * Q_PARTS * 2 * Q_STRIDE / 4; i += 32 * SCORE_WARPS)  // the two columns that are no head
     *(uint32_t*)&sq[i / (2 * Q_STRIDE / 4) * (8 * Q_STRIDE) + 6 * Q_STRIDE + i % (2 * Q_STRIDE / 4) * 4] = 0;
   pdl_wait();
   const int nb = blocks_of(p.c, b, T - 1), ngroups = (nb + SCORE_GROUP - 1) / SCORE_GROUP;
   if (nb <= p.k || (int)blockIdx.x >= ngroups) return;  // every block is taken; or no block of this sequence
-  uint4 lo[2][8], hi[2][8];  // rows g and g + 8, 32 dims each: 8 of them in this lane
-  bool there[2];
-  auto load = [&](int group) {
+  uint4 lo[2][PER], hi[2][PER];  // a turn's dims of rows g and g + 8, 32 dims each: 8 of them in this lane
+  int64_t at[2];
+  auto aim = [&](int group) {
 #pragma unroll
     for (int e = 0; e < 2; e++) {
       const int blk = group * SCORE_GROUP + 16 * warp + g + 8 * e;
-      const int64_t at = blk < nb ? bounds_index(p.c, b, kh, blk) : -1;
-      there[e] = at >= 0;
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        lo[e][j] = hi[e][j] = make_uint4(0, 0, 0, 0);
-        if (at >= 0) {
-          lo[e][j] = *(const uint4*)(p.bounds + at * 2 * AD + 32 * j + 8 * tg);
-          hi[e][j] = *(const uint4*)(p.bounds + at * 2 * AD + AD + 32 * j + 8 * tg);
-        }
-      }
+      at[e] = blk < nb ? bounds_index(p.c, b, kh, blk) : -1;
     }
   };
-  load(blockIdx.x);
+  auto load = [&](int turn) {
+#pragma unroll
+    for (int e = 0; e < 2; e++)
+#pragma unroll
+      for (int j = 0; j < PER; j++) {
+        lo[e][j] = hi[e][j] = make_uint4(0, 0, 0, 0);
+        if (at[e] >= 0) {
+          lo[e][j] = *(const uint4*)(p.bounds + at[e] * 2 * AD + 32 * PER * turn + 32 * j + 8 * tg);
+          hi[e][j] = *(const uint4*)(p.bounds + at[e] * 2 * AD + AD + 32 * PER * turn + 32 * j + 8 * tg);
+        }
+      }
+  };
+  aim(blockIdx.x);
+  load(0);
   for (int i = warp; i < T * GQA; i += SCORE_WARPS) {
     const int t = i / GQA, h = i % GQA;
     const float* src = p.qn + (((size_t)b * T + t) * nqh + kh * GQA + h) * AD + 8 * lane;
@@ -260,36 +266,48 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const Select
   __syncthreads();
 #pragma unroll 1
   for (int group = blockIdx.x; group < ngroups; group += gridDim.x) {
-    if (group != (int)blockIdx.x) load(group);
+    if (group != (int)blockIdx.x) {
+      aim(group);
+      load(0);
+    }
     const int ahead = (group + gridDim.x) * SCORE_GROUP + 16 * warp + (lane >> 1);  // the next group's bounds into L2, half a block a lane
     if (ahead < nb) {
-      const int64_t at = bounds_index(p.c, b, kh, ahead);
-      if (at >= 0)
+      const int64_t next = bounds_index(p.c, b, kh, ahead);
+      if (next >= 0)
 #pragma unroll
-        for (int i = 0; i < 4; i++) prefetch_l2(p.bounds + at * 2 * AD + (lane & 1) * AD + 64 * i);
+        for (int i = 0; i < 4; i++) prefetch_l2(p.bounds + next * 2 * AD + (lane & 1) * AD + 64 * i);
     }
+    float sp[T][4] = {}, sm[T][4] = {}, sl[T][4] = {}, sn[T][4] = {}, sa[T][4] = {};
 #pragma unroll 1
-    for (int t = 0; t < T; t++) {
-      const uint8_t* qt = sq + t * Q_TOKEN + g * Q_STRIDE + 16 * tg;
-      float sp[4] = {}, sm[4] = {}, sl[4] = {}, sn[4] = {}, sa[4] = {};
+    for (int turn = 0; turn < TURNS; turn++) {
+      if (turn) load(turn);
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        uint4 q[Q_PARTS];
-#pragma unroll
-        for (int k = 0; k < Q_PARTS; k++) q[k] = *(const uint4*)(qt + k * 8 * Q_STRIDE + 64 * j);
+      for (int j = 0; j < PER; j++) {
         const uint4 l0 = lo[0][j], l1 = lo[1][j], h0 = hi[0][j], h1 = hi[1][j];
-        mma16816(sp, h0.x, h1.x, h0.y, h1.y, q[QP_HI].x, q[QP_HI].y);
-        mma16816(sm, l0.x, l1.x, l0.y, l1.y, q[QM_HI].x, q[QM_HI].y);
-        mma16816(sl, h0.x, h1.x, h0.y, h1.y, q[QP_LO].x, q[QP_LO].y);
-        mma16816(sp, h0.z, h1.z, h0.w, h1.w, q[QP_HI].z, q[QP_HI].w);
-        mma16816(sm, l0.z, l1.z, l0.w, l1.w, q[QM_HI].z, q[QM_HI].w);
-        mma16816(sn, l0.x, l1.x, l0.y, l1.y, q[QM_LO].x, q[QM_LO].y);
-        mma16816(sl, h0.z, h1.z, h0.w, h1.w, q[QP_LO].z, q[QP_LO].w);
-        mma16816(sn, l0.z, l1.z, l0.w, l1.w, q[QM_LO].z, q[QM_LO].w);
         const auto widest = [](uint32_t x, uint32_t y) { return h2_as_u32(__hmax2_nan(__habs2(u32_as_h2(x)), __habs2(u32_as_h2(y)))); };
-        mma16816(sa, widest(l0.x, h0.x), widest(l1.x, h1.x), widest(l0.y, h0.y), widest(l1.y, h1.y), q[QABS].x, q[QABS].y);
-        mma16816(sa, widest(l0.z, h0.z), widest(l1.z, h1.z), widest(l0.w, h0.w), widest(l1.w, h1.w), q[QABS].z, q[QABS].w);
+        const uint4 w0 = make_uint4(widest(l0.x, h0.x), widest(l0.y, h0.y), widest(l0.z, h0.z), widest(l0.w, h0.w));
+        const uint4 w1 = make_uint4(widest(l1.x, h1.x), widest(l1.y, h1.y), widest(l1.z, h1.z), widest(l1.w, h1.w));
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+          const uint8_t* qt = sq + t * Q_TOKEN + g * Q_STRIDE + 16 * tg + 64 * PER * turn + 64 * j;
+          uint4 q[Q_PARTS];
+#pragma unroll
+          for (int k = 0; k < Q_PARTS; k++) q[k] = *(const uint4*)(qt + k * 8 * Q_STRIDE);
+          mma16816(sp[t], h0.x, h1.x, h0.y, h1.y, q[QP_HI].x, q[QP_HI].y);
+          mma16816(sm[t], l0.x, l1.x, l0.y, l1.y, q[QM_HI].x, q[QM_HI].y);
+          mma16816(sl[t], h0.x, h1.x, h0.y, h1.y, q[QP_LO].x, q[QP_LO].y);
+          mma16816(sn[t], l0.x, l1.x, l0.y, l1.y, q[QM_LO].x, q[QM_LO].y);
+          mma16816(sa[t], w0.x, w1.x, w0.y, w1.y, q[QABS].x, q[QABS].y);
+          mma16816(sp[t], h0.z, h1.z, h0.w, h1.w, q[QP_HI].z, q[QP_HI].w);
+          mma16816(sm[t], l0.z, l1.z, l0.w, l1.w, q[QM_HI].z, q[QM_HI].w);
+          mma16816(sl[t], h0.z, h1.z, h0.w, h1.w, q[QP_LO].z, q[QP_LO].w);
+          mma16816(sn[t], l0.z, l1.z, l0.w, l1.w, q[QM_LO].z, q[QM_LO].w);
+          mma16816(sa[t], w0.z, w1.z, w0.w, w1.w, q[QABS].z, q[QABS].w);
+        }
       }
+    }
+#pragma unroll
+    for (int t = 0; t < T; t++) {
       // rows g and g + 8, heads 2 tg and 2 tg + 1
 #pragma unroll
       for (int e = 0; e < 2; e++) {
@@ -298,7 +316,7 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const Select
         if (tg < 3) {
 #pragma unroll
           for (int i = 0; i < 2; i++) {
-            const float u = unit[t][2 * tg + i], v = (sp[2 * e + i] + sm[2 * e + i] + (sl[2 * e + i] + sn[2 * e + i])) * u, a = sa[2 * e + i] * u * 6.2e-5f;
+            const float u = unit[t][2 * tg + i], v = (sp[t][2 * e + i] + sm[t][2 * e + i] + (sl[t][2 * e + i] + sn[t][2 * e + i])) * u, a = sa[t][2 * e + i] * u * 6.2e-5f;
             odd |= !(fabsf(v) <= 3e38f) || !(a <= 3e38f);
             best = fmaxf(best, v);
             err = fmaxf(err, a);
@@ -312,7 +330,7 @@ __global__ void __launch_bounds__(32 * SCORE_WARPS, 2) score_kernel(const Select
         }
         const int blk = group * SCORE_GROUP + 16 * warp + g + 8 * e;
         if (tg == 0 && blk < nb)
-          p.score[(((size_t)b * T + t) * p.c.nkvh + kh) * p.max_blocks + blk] = there[e] ? make_float2(best, err) : make_float2(-3e38f, 0.f);
+          p.score[(((size_t)b * T + t) * p.c.nkvh + kh) * p.max_blocks + blk] = at[e] >= 0 ? make_float2(best, err) : make_float2(-3e38f, 0.f);
       }
     }
   }
@@ -600,7 +618,10 @@ int launch_select(DeviceCtx* ctx, SelectParams& p, int max_len, const char* who,
     std::lock_guard<std::mutex> lock(attr_mu);
     if (!attr[ctx->dev]) {
       Q27B_CK(cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(SEL_MAX_BLOCKS)));
-      Q27B_CK(cudaFuncSetAttribute(score_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Q27B_MAX_T * Q_TOKEN));
+      Q27B_CK(cudaFuncSetAttribute(score_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, 1 * Q_TOKEN));
+      Q27B_CK(cudaFuncSetAttribute(score_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * Q_TOKEN));
+      Q27B_CK(cudaFuncSetAttribute(score_kernel<3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * Q_TOKEN));
+      Q27B_CK(cudaFuncSetAttribute(score_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * Q_TOKEN));
       attr[ctx->dev] = true;
     }
   }
@@ -624,7 +645,8 @@ int launch_select(DeviceCtx* ctx, SelectParams& p, int max_len, const char* who,
     // goes through several groups of 64 blocks with the queries staged once.
     const int64_t pairs = (int64_t)p.c.nkvh * p.c.B, groups = (p.max_blocks + SCORE_GROUP - 1) / SCORE_GROUP;
     const int64_t ctas = std::max<int64_t>(1, std::min<int64_t>(groups, (4 * (int64_t)ctx->n_sm + pairs - 1) / pairs));
-    Q27B_CK(launch_step(score_kernel, dim3((unsigned)ctas, p.c.nkvh, p.c.B), dim3(32 * SCORE_WARPS), p.c.T * Q_TOKEN, s, p));
+    auto* score = p.c.T == 1 ? score_kernel<1> : p.c.T == 2 ? score_kernel<2> : p.c.T == 3 ? score_kernel<3> : score_kernel<4>;
+    Q27B_CK(launch_step(score, dim3((unsigned)ctas, p.c.nkvh, p.c.B), dim3(32 * SCORE_WARPS), p.c.T * Q_TOKEN, s, p));
   }
   Q27B_CK(launch_step(select_kernel, dim3(p.c.nkvh, p.c.T, p.c.B), dim3(SEL_THREADS), scored ? smem_of(p.max_blocks) : 0, s, p));
   return Q27B_OK;
