@@ -16,8 +16,8 @@
  * (see q27b_attn_workspace_*): a status word, the decode partials (fixed size, allocated by the
  * first decode call), the prefill partials (allocated once, by the first prefill call that splits,
  * at a fixed cap - a later, deeper call splits less instead of reallocating, as the reference's
- * fixed buffer, src/attn.cu:954-959) and the partials of the batched paged decode (grow with the
- * batch). Run every shape class once before capturing a CUDA graph (the reference's
+ * fixed buffer, src/attn.cu:954-959) and the partials of the calls over pages (grow with the
+ * batch; what they were in before stays allocated, since captured graphs may name it). Run every shape class once before capturing a CUDA graph (the reference's
  * Decoder::warmup does the same, src/model.cu:910-931), or fix everything up front with
  * q27b_attn_workspace_init.
  * Threading: one caller thread per device at a time (as the reference, src/attn.cu:869-879);
@@ -432,9 +432,10 @@ int q27b_prefill_qk_debug(const float* x, int rows, float kq_scale, const void* 
  * (rope3[t] = pos0 + depth[t], three times), q27b_attn_decode_tree attends, the caller samples and finds the accepted path,
  * q27b_kv_commit moves its rows to the front, q27b_kv_bounds brings the blocks' bounds up to date. A draft step with few
  * blocks: q27b_attn_prep, q27b_kv_bounds, q27b_select_blocks, q27b_attn_decode_blocks.
- * All of them keep their scratch in the workspace: one stream order per device, as for the other entry points. Indices that
- * the device finds out of range are skipped and reported in the device status word (bit 1: page table, bit 2: path or list
- * of blocks). */
+ * Their scratch lies in the workspace, of one sequence in the prefill buffer (at its fixed size; a smaller one makes for fewer
+ * parts, or Q27B_UNSUPPORTED), over pages in the paged buffer: calls that can overlap on the GPU race on it, so keep those of
+ * one device in one stream order. Float and cache pointers lie on 16-byte boundaries. Indices that the device finds out of
+ * range are skipped and reported in the device status word (bit 1: page table, bit 2: path or list of blocks). */
 
 /* Masks and depths of a tree of T = 1..64 drafts in which parent[t] is the draft before t (smaller than t) or -1 for a
  * child of the last accepted token: mask[t] has bit j set for j = t and every ancestor j of t, depth[t] (may be null)
@@ -472,7 +473,8 @@ int q27b_kv_commit_paged(void* kpool, void* vpool, const int* page_table, const 
  * reads it (f16; q8_0: value times scale). Layout f16 [nkvh][ceil(n_ctx / 64)][2][256] beside a contiguous cache,
  * [n_pages][nkvh][4][2][256] beside a K pool. The call writes the bounds of every block that holds one of the rows
  * *pos0 .. *pos0 + T - 1 (paged: seq_len[b] - T ..), over all rows of the block below *pos0 + T: after an append, a commit
- * or a prompt's chunk, or of the whole cache at once. NaN in a key makes its bound NaN. */
+ * or a prompt's chunk, or of the whole cache at once. NaN in a key makes its bound NaN. Pages that sequences share share their
+ * bounds; q27b_kv_page_copy copies none (bring the new page's up to date with this call). */
 uint64_t q27b_kv_bounds_bytes(int nkvh, int n_ctx);
 uint64_t q27b_kv_bounds_pool_bytes(int nkvh, int n_pages);
 int q27b_kv_bounds(const void* kcache, void* bounds, const int* pos0, int T, int nkvh, int n_ctx, int q8, void* stream);

@@ -138,10 +138,10 @@ int launch_rows_merge(const RowsParams& p, int64_t rows, int n_sm, cudaStream_t 
 
 // Room for the partials of `rows` rows (and `more` floats behind them): in the prefill workspace, whose size is fixed, or, for a
 // batch, in the paged workspace. *fit: as many of `rows` as there is room for (a batch: all).
-int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t more, int64_t* fit, float** part) {
+int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t more, int64_t* fit, float** part, const char* who) {
   const size_t floats = (size_t)rows * (AD + 2) + (size_t)more;
   *fit = rows;
-  if (p.c.page_table) return paged_ws(ctx, floats, part);
+  if (p.c.page_table) return paged_ws(ctx, floats, part, who);
   size_t cap;
   if (int rc = prefill_ws(ctx, part, &cap)) return rc;
   if (cap < floats) *fit = cap < (size_t)more ? 0 : (int64_t)((cap - (size_t)more) / (AD + 2));
@@ -187,7 +187,7 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   const WsGroups groups = plan.groups;
   float* part;
   int64_t fit;
-  if (int rc = place_partials(ctx, p, rows * nch, 0, &fit, &part)) return rc;
+  if (int rc = place_partials(ctx, p, rows * nch, 0, &fit, &part, who)) return rc;
   if (fit < rows) return no_room(who);
   const int chunk = (p.k + (int)(fit / rows) - 1) / (int)(fit / rows);
   if (chunk > SEL_CHUNK) return no_room(who);
@@ -221,7 +221,7 @@ int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   int64_t parts = std::max<int64_t>(1, std::min<int64_t>(ctx->n_sm / units, tree_tiles(p.c.n_ctx))), fit;
   int64_t slots = paged ? tree_grid(units, ctx->n_sm) : units * parts;
   float* part;
-  if (int rc = place_partials(ctx, p, slots * TREE_ROWS, head, &fit, &part)) return rc;
+  if (int rc = place_partials(ctx, p, slots * TREE_ROWS, head, &fit, &part, who)) return rc;
   if (fit < slots * TREE_ROWS) {
     parts = fit / (units * TREE_ROWS);
     if (parts < 1) return no_room(who);
@@ -265,6 +265,7 @@ int q27b_attn_decode_tree(const float* qn, const float* qg, const void* kcache, 
     return fail(Q27B_BAD_SHAPE, "attn_decode_tree: bad shape");
   if (!qn || !qg || !kcache || !vcache || !pos0 || !mask || (!o && !xq) || (xq && !xd))
     return fail(Q27B_BAD_SHAPE, "attn_decode_tree: null pointer");
+  if (misaligned({qn, qg, kcache, vcache, o, xq})) return fail(Q27B_BAD_SHAPE, "attn_decode_tree: pointers must be 16-byte aligned");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
   RowsParams p = {};
@@ -281,6 +282,7 @@ int q27b_attn_decode_tree_paged(const float* qn, const float* qg, const void* kp
     return fail(Q27B_BAD_SHAPE, "attn_decode_tree_paged: bad shape");
   if (!qn || !qg || !kpool || !vpool || !page_table || !seq_len || !mask || (!o && !xq) || (xq && !xd))
     return fail(Q27B_BAD_SHAPE, "attn_decode_tree_paged: null pointer");
+  if (misaligned({qn, qg, kpool, vpool, o, xq})) return fail(Q27B_BAD_SHAPE, "attn_decode_tree_paged: pointers must be 16-byte aligned");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
   RowsParams p = {};
@@ -299,6 +301,7 @@ int q27b_attn_decode_blocks(const float* qn, const float* qg, const void* kcache
     return fail(Q27B_BAD_SHAPE, "attn_decode_blocks: bad shape");
   if (!qn || !qg || !kcache || !vcache || !pos0 || !sel || (!o && !xq) || (xq && !xd))
     return fail(Q27B_BAD_SHAPE, "attn_decode_blocks: null pointer");
+  if (misaligned({qn, qg, kcache, vcache, o, xq})) return fail(Q27B_BAD_SHAPE, "attn_decode_blocks: pointers must be 16-byte aligned");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
   RowsParams p = {};
@@ -316,6 +319,7 @@ int q27b_attn_decode_blocks_paged(const float* qn, const float* qg, const void* 
     return fail(Q27B_BAD_SHAPE, "attn_decode_blocks_paged: bad shape");
   if (!qn || !qg || !kpool || !vpool || !page_table || !seq_len || !sel || (!o && !xq) || (xq && !xd))
     return fail(Q27B_BAD_SHAPE, "attn_decode_blocks_paged: null pointer");
+  if (misaligned({qn, qg, kpool, vpool, o, xq})) return fail(Q27B_BAD_SHAPE, "attn_decode_blocks_paged: pointers must be 16-byte aligned");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
   RowsParams p = {};

@@ -95,9 +95,20 @@ int prefill_ws(DeviceCtx* ctx, float** out, size_t* max_floats) {
   return Q27B_OK;
 }
 
-int paged_ws(DeviceCtx* ctx, size_t floats, float** out) {
-  if (ctx->paged.floats < floats)
-    if (int rc = alloc_ws(ctx, &ctx->paged, floats, "attn_decode_paged")) return rc;
+int paged_ws(DeviceCtx* ctx, size_t floats, float** out, const char* who) {
+  if (ctx->paged.floats < floats) {
+    WsBuf next;
+    if (!ctx->frozen) floats = std::max(floats, ctx->paged.floats + ctx->paged.floats / 2);
+    else next.floats = ctx->paged.floats;  // (for the message)
+    try {
+      ctx->outgrown.reserve(ctx->outgrown.size() + 1);
+    } catch (const std::exception&) {
+      return fail(Q27B_CUDA_ERROR, std::string(who) + ": out of host memory");
+    }
+    if (int rc = alloc_ws(ctx, &next, floats, who)) return rc;
+    if (ctx->paged.p) ctx->outgrown.push_back(ctx->paged.p);
+    ctx->paged = next;
+  }
   *out = ctx->paged.p;
   return Q27B_OK;
 }
@@ -268,6 +279,8 @@ int q27b_attn_workspace_destroy(void) {
     b->p = nullptr;
     b->floats = 0;
   }
+  for (float* p : ctx->outgrown) Q27B_CK(cudaFree(p));
+  ctx->outgrown.clear();
   if (ctx->ref_scores) Q27B_CK(cudaFree(ctx->ref_scores));
   ctx->ref_scores = nullptr;
   ctx->ref_scores_floats = 0;

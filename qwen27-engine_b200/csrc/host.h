@@ -6,7 +6,9 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 #include <string>
+#include <vector>
 
 #include "../../include/q27b_attn.h"
 
@@ -40,7 +42,8 @@ struct DeviceCtx {
   // names (the reference keeps its prefill buffer apart and fixed for the same reason, src/attn.cu:954-959):
   WsBuf dec;                  // decode of one sequence: n_sm chunk partials, fixed size, allocated on first use
   WsBuf pf;                   // prefill: allocated once at pf_cap_floats; the split count is cut to fit
-  WsBuf paged;                // batched decode: grows with the batch unless the workspace is frozen
+  WsBuf paged;                // calls over pages: grows with the batch unless the workspace is frozen
+  std::vector<float*> outgrown;  // what `paged` was before: captured graphs may name it, so it stays until the workspace is destroyed
   size_t pf_cap_floats = 0;   // 0: default (see workspace_defaults in host.cu)
   bool frozen = false;        // after q27b_attn_workspace_init: nothing may be allocated any more
   float* ref_scores = nullptr;  // scratch of the slow checking kernel (q27b_attn_decode_ref), grown on demand
@@ -58,9 +61,15 @@ int device_ctx(DeviceCtx** out);
 int decode_ws(DeviceCtx* ctx, float** out);
 // The prefill partial buffer, allocated once at its cap. *max_floats = its size.
 int prefill_ws(DeviceCtx* ctx, float** out, size_t* max_floats);
-// The batched-decode partial buffer with room for `floats`; grows (free + allocate) when it has to,
-// unless the workspace is frozen, in which case a larger request fails with Q27B_UNSUPPORTED.
-int paged_ws(DeviceCtx* ctx, size_t floats, float** out);
+// The buffer of the calls over pages with room for `floats`; grows when it has to (to half as much again at least; the old one
+// stays allocated), unless the workspace is frozen, in which case a larger request of `who` fails with Q27B_UNSUPPORTED.
+int paged_ws(DeviceCtx* ctx, size_t floats, float** out, const char* who = "attn_decode_paged");
+// Whether one of the addresses is not on a 16-byte boundary (null is): the kernels load and store 16 bytes at a time.
+inline bool misaligned(std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if ((uintptr_t)p & 15) return true;
+  return false;
+}
 // Cuts a prefill split plan (ts tiles, `tokens` tokens, cut into ns pieces) to what the prefill buffer holds: fewer pieces, or no split at all; must_merge (q8_1 through the merge kernel) fails
 // instead when not even two pieces fit.
 int fit_prefill_split(DeviceCtx* ctx, int* ts, int* ns, int tokens, int nqh, bool must_merge, float** part);

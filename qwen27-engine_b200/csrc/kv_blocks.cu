@@ -686,7 +686,7 @@ int launch_select(DeviceCtx* ctx, SelectParams& p, int max_len, const char* who,
     const size_t floats = (size_t)p.c.B * p.c.T * p.c.nkvh * p.max_blocks * 2;
     float* scratch;
     if (p.c.page_table) {
-      if (int rc = paged_ws(ctx, floats, &scratch)) return rc;
+      if (int rc = paged_ws(ctx, floats, &scratch, who)) return rc;
     } else {
       size_t cap;
       if (int rc = prefill_ws(ctx, &scratch, &cap)) return rc;
@@ -726,6 +726,7 @@ extern "C" {
 int q27b_kv_commit(void* kcache, void* vcache, const int* pos0, const int* path, const int* count, int T, int nkvh, int n_ctx,
                    int q8, void* stream) {
   if (!kcache || !vcache || !pos0 || !path || !count) return fail(Q27B_BAD_SHAPE, "kv_commit: null pointer");
+  if (misaligned({kcache, vcache})) return fail(Q27B_BAD_SHAPE, "kv_commit: pointers must be 16-byte aligned");
   if (bad_contiguous(T, MAX_TREE_T, nkvh, n_ctx)) return fail(Q27B_BAD_SHAPE, "kv_commit: bad shape");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
@@ -735,6 +736,7 @@ int q27b_kv_commit(void* kcache, void* vcache, const int* pos0, const int* path,
 int q27b_kv_commit_paged(void* kpool, void* vpool, const int* page_table, const int* seq_len, const int* path, const int* count,
                          int B, int T, int nkvh, int n_pages, int max_pages, void* stream) {
   if (!kpool || !vpool || !page_table || !seq_len || !path || !count) return fail(Q27B_BAD_SHAPE, "kv_commit_paged: null pointer");
+  if (misaligned({kpool, vpool})) return fail(Q27B_BAD_SHAPE, "kv_commit_paged: pointers must be 16-byte aligned");
   if (bad_paged(B, T, MAX_TREE_T, nkvh, n_pages, max_pages)) return fail(Q27B_BAD_SHAPE, "kv_commit_paged: bad shape");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
@@ -751,6 +753,7 @@ uint64_t q27b_kv_bounds_pool_bytes(int nkvh, int n_pages) {
 
 int q27b_kv_bounds(const void* kcache, void* bounds, const int* pos0, int T, int nkvh, int n_ctx, int q8, void* stream) {
   if (!kcache || !bounds || !pos0) return fail(Q27B_BAD_SHAPE, "kv_bounds: null pointer");
+  if (misaligned({kcache, bounds})) return fail(Q27B_BAD_SHAPE, "kv_bounds: pointers must be 16-byte aligned");
   if (bad_contiguous(T, 0x7fffffff, nkvh, n_ctx) || T > n_ctx) return fail(Q27B_BAD_SHAPE, "kv_bounds: bad shape");
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
@@ -760,6 +763,7 @@ int q27b_kv_bounds(const void* kcache, void* bounds, const int* pos0, int T, int
 int q27b_kv_bounds_paged(const void* kpool, void* bounds, const int* page_table, const int* seq_len, int B, int T, int nkvh,
                          int n_pages, int max_pages, void* stream) {
   if (!kpool || !bounds || !page_table || !seq_len) return fail(Q27B_BAD_SHAPE, "kv_bounds_paged: null pointer");
+  if (misaligned({kpool, bounds})) return fail(Q27B_BAD_SHAPE, "kv_bounds_paged: pointers must be 16-byte aligned");
   if (bad_paged(B, T, 0x7fffffff, nkvh, n_pages, max_pages) || T > max_pages * Q27B_PAGE)
     return fail(Q27B_BAD_SHAPE, "kv_bounds_paged: bad shape");
   DeviceCtx* ctx;
@@ -771,6 +775,7 @@ int q27b_kv_bounds_paged(const void* kpool, void* bounds, const int* page_table,
 int q27b_select_blocks(const float* qn, const void* bounds, int* sel, const int* pos0, int T, int k, int n_sink, int n_recent,
                        int nqh, int nkvh, int n_ctx, void* stream) {
   if (!qn || !bounds || !sel || !pos0) return fail(Q27B_BAD_SHAPE, "select_blocks: null pointer");
+  if (misaligned({bounds})) return fail(Q27B_BAD_SHAPE, "select_blocks: pointers must be 16-byte aligned");
   if (bad_contiguous(T, Q27B_MAX_T, nkvh, n_ctx)) return fail(Q27B_BAD_SHAPE, "select_blocks: bad shape");
   if (int rc = check_select("select_blocks", T, k, n_sink, n_recent, nqh, nkvh, n_ctx)) return rc;
   DeviceCtx* ctx;
@@ -785,6 +790,7 @@ int q27b_select_blocks_paged(const float* qn, const void* bounds, int* sel, cons
                              int T, int k, int n_sink, int n_recent, int nqh, int nkvh, int n_pages, int max_pages,
                              int max_seq_len, void* stream) {
   if (!qn || !bounds || !sel || !page_table || !seq_len) return fail(Q27B_BAD_SHAPE, "select_blocks_paged: null pointer");
+  if (misaligned({bounds})) return fail(Q27B_BAD_SHAPE, "select_blocks_paged: pointers must be 16-byte aligned");
   if (bad_paged(B, T, Q27B_MAX_T, nkvh, n_pages, max_pages) || max_seq_len < T || max_seq_len > max_pages * Q27B_PAGE)
     return fail(Q27B_BAD_SHAPE, "select_blocks_paged: bad shape");
   if (int rc = check_select("select_blocks_paged", T, k, n_sink, n_recent, nqh, nkvh, max_seq_len)) return rc;

@@ -289,3 +289,137 @@ def test_commit_reports_what_is_no_draft(q27):
         assert torch.equal(v[ok], bv[ok])
         kc.copy_(before)
     assert q27.device_status() == 0
+
+
+# ---------------------------------------------------------------- memory
+def test_rows_far_behind_2_to_the_31_bytes(q27):
+    """Pages at both ends of a pool of 2.7 GB: addresses and row numbers that 32 bits of bytes do not reach."""
+    n_pages, nkvh, T = 39000, 1, 7
+    st = H.Store([600], T, nkvh, True, True, seed=1, extra_pages=0)
+    st.n_pages, st.rows = n_pages, n_pages * nkvh * H.PAGE
+    st.host_table = [[n_pages - 1, 0, n_pages - 17]]
+    st.table = H.i32(st.host_table)
+    kc, vc = (torch.empty(st.rows * (H.AD + 16), dtype=torch.uint8, device="cuda") for _ in range(2))
+    assert kc.numel() > 2 ** 31
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    masks = H.random_masks(1, T, seed=2)
+    qn, qg = H.queries(st, 3)
+    o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+    H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+    rows = lambda buf, pos: tuple(x.clone() for x in (st.parts(buf)[0][st.index(0, 0, pos)], st.parts(buf)[1][st.index(0, 0, pos)]))  # noqa: E731
+    want = [rows(c, [600 - T + 3, 600 - T + 5]) for c in (kc, vc)]
+    q27.kv_commit_paged(kc, vc, st.table, st.seq_len, H.i32([[3, 5, 0, 0, 0, 0, 0]]), H.i32([2]), 1, T, nkvh, n_pages, st.max_pages)
+    got = [rows(c, [600 - T, 600 - T + 1]) for c in (kc, vc)]
+    for a, b in zip(want, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    bounds = torch.full((n_pages * 4, 2, H.AD), 7.5, dtype=torch.float16, device="cuda")
+    H.call_bounds(q27, st, kc, bounds, 600)
+    for blk in range(10):
+        x = st.read(kc, 0, 0, range(64 * blk, min(600, 64 * blk + 64))).half()
+        i = H.bounds_at(st, 0, 0, blk)
+        assert torch.equal(bounds[i, 0], x.amin(0)) and torch.equal(bounds[i, 1], x.amax(0))
+    st1 = H.Store([600], 1, nkvh, True, True, seed=1, extra_pages=0)
+    st1.n_pages, st1.rows, st1.table, st1.host_table = n_pages, st.rows, st.table, st.host_table
+    q1, g1 = H.queries(st1, 4)
+    sel = H.call_select(q27, st1, q1, bounds, 5, 1, 2)
+    assert torch.equal(sel.cpu(), H.select_reference(st1, q1, bounds, 5, 1, 2))
+    o = H.call_blocks(q27, st1, kc, vc, q1, g1, sel)
+    pos = lambda b, t, h: [p for x in sel[0, 0, h].tolist() for p in range(64 * x, min(64 * x + 64, 600))]  # noqa: E731
+    H.check_attention(o, H.attention(st1, kc, vc, q1, g1, pos))
+    assert q27.device_status() == 0
+
+
+def test_small_and_fixed_workspaces(q27):
+    """A prefill buffer that holds fewer parts gives the same result; one that holds none, and a paged buffer that is fixed and
+    too small, are refused with the caller's name. A paged buffer that grows leaves what a captured graph names in place."""
+    T = 9
+    st = H.Store([1500], T, 2, False, True, seed=4)
+    pg = H.Store([1500, 700], T, 2, True, True, seed=4)
+    sets = []
+    for s in (st, pg):
+        kc, vc = s.new(), s.new()
+        s.fill(kc, H.gen(1))
+        s.fill(vc, H.gen(2))
+        masks = H.random_masks(s.B, T, seed=1)
+        qn, qg = H.queries(s, 3)
+        sets.append((s, kc, vc, qn, qg, H.mask_tensor(masks), H.attention(s, kc, vc, qn, qg, H.tree_visible(s, masks))))
+    sel = torch.tensor([[[[0, 3, 9], [1, 2, 3]]]], dtype=torch.int32, device="cuda")
+    st1 = H.Store([1500], 1, 2, False, True, seed=4, n_ctx=st.n_ctx)
+    try:
+        q27.workspace_destroy()
+        q27.workspace_init(2 * 3 * 128 * 258 * 4 + 64, 4096)  # three parts for each of the two units
+        H.check_attention(H.call_tree(q27, *sets[0][:6]), sets[0][6])
+        with pytest.raises(q27.Q27Error, match="attn_decode_tree_paged.*fixed"):
+            H.call_tree(q27, *sets[1][:6])
+        q27.workspace_destroy()
+        q27.workspace_init(4096, 0)
+        with pytest.raises(q27.Q27Error, match="attn_decode_tree: the prefill workspace is too small"):
+            H.call_tree(q27, *sets[0][:6])
+        with pytest.raises(q27.Q27Error, match="attn_decode_blocks: the prefill workspace is too small"):
+            H.call_blocks(q27, st1, sets[0][1], sets[0][2], sets[0][3][:, :1].contiguous(), sets[0][4][:, :1].contiguous(), sel)
+        q27.workspace_destroy()
+        # over pages: a graph, then a call that needs more
+        o = H.call_tree(q27, *sets[1][:6])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            H.call_tree(q27, *sets[1][:6], o)
+        before = q27.workspace_query()[2]
+        big = H.Store([300] * 40, 64, 4, True, True, seed=4)
+        kb, vb = big.new(), big.new()
+        big.fill(kb, H.gen(1))
+        big.fill(vb, H.gen(2))
+        qn, qg = H.queries(big, 3)
+        H.call_tree(q27, big, kb, vb, qn, qg, H.mask_tensor(H.random_masks(40, 64, seed=1)))
+        assert q27.workspace_query()[2] > before
+        o.zero_()
+        graph.replay()
+        H.check_attention(o, sets[1][6])
+        assert q27.device_status() == 0
+    finally:
+        torch.cuda.synchronize()
+        q27.workspace_destroy()
+
+
+def test_tensors_that_are_too_small_or_elsewhere(q27):
+    st = H.Store([100], 6, 2, False, True, seed=1)
+    kc, vc = st.new(), st.new()
+    qn, qg = H.queries(st, 3)
+    o = torch.zeros((6, 12, H.AD), dtype=torch.float16, device="cuda")
+    mask = torch.zeros(6, dtype=torch.int64, device="cuda")
+    good = [qn, qg, kc, vc, o, None, None, st.pos0, mask]
+    nums = (6, H.SCALE, 12, 2, st.n_ctx)
+    for i, name in ((0, "elements"), (1, "elements"), (2, "bytes"), (3, "bytes"), (4, "elements"), (8, "elements")):
+        bad = list(good)
+        bad[i] = good[i].flatten()[:-16 if i != 8 else -1]
+        with pytest.raises(q27.Q27Error, match="expected at least .* " + name):
+            q27.attn_decode_tree(*bad, *nums)
+    for i, other in ((0, qn.half()), (4, o.float()), (7, st.pos0.long()), (8, mask.int())):
+        bad = list(good)
+        bad[i] = other
+        with pytest.raises(q27.Q27Error, match="expected dtype"):
+            q27.attn_decode_tree(*bad, *nums)
+    bad = list(good)
+    bad[0] = torch.zeros(qn.numel() + 1, device="cuda")[1:]
+    with pytest.raises(q27.Q27Error, match="16-byte aligned"):
+        q27.attn_decode_tree(*bad, *nums)
+    with pytest.raises(q27.Q27Error, match="contiguous"):
+        q27.attn_decode_tree(qn.expand(2, 6, 12, H.AD), *good[1:], *nums)
+
+
+@pytest.mark.parametrize("mode", ["0", "1"])
+def test_other_launch_modes(q27, mode):
+    """Without programmatic launches, and with every kernel launched that way."""
+    import os
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    subset = ["tests/test_gpu_tree.py::test_against_64_bits", "tests/test_gpu_tree.py::test_replayed_graph_sees_new_positions_and_masks",
+              "tests/test_gpu_blocks.py::test_a_speculative_step", "tests/test_gpu_blocks.py::test_all_blocks_are_attn_decode",
+              "tests/test_gpu_blocks.py::test_blocks_against_64_bits"]
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider"] + subset, cwd=ROOT,
+                       env=dict(os.environ, Q27_PDL=mode), capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-1000:]
+    assert " passed" in r.stdout

@@ -82,6 +82,22 @@ def test_null_pointers_are_refused(q27, lib, name):
         assert call(lib, name, {"xq": ONE}) == q27.BAD_SHAPE  # without xd
 
 
+@pytest.mark.parametrize("name", CALLS)
+def test_addresses_between_boundaries_are_refused(q27, lib, name):
+    """The kernels load and store 16 bytes at a time."""
+    wide = [p.rstrip("?") for p in CALLS[name][0] if p.rstrip("?") in ("qn", "qg", "kc", "vc", "kp", "vp", "o", "xq", "bounds")]
+    if name.startswith("select"):
+        wide.remove("qn")  # read value by value
+    assert wide
+    for p in wide:
+        for off in (4, 8, 12):
+            ptrs = {p: ctypes.c_void_p(16 + off)}
+            if p == "xq":
+                ptrs["xd"] = ONE
+            assert call(lib, name, ptrs) == q27.BAD_SHAPE, p
+            assert ("%s: pointers must be 16-byte aligned" % name).encode() in lib.q27b_last_error()
+
+
 def test_sizes_of_the_bounds(q27):
     assert q27.kv_bounds_bytes(4, 1000) == 4 * 16 * 1024
     assert q27.kv_bounds_bytes(2, 64) == 2 * 1024 and q27.kv_bounds_bytes(2, 65) == 4 * 1024
