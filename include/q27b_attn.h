@@ -433,9 +433,11 @@ int q27b_prefill_qk_debug(const float* x, int rows, float kq_scale, const void* 
  * q27b_kv_commit moves its rows to the front, q27b_kv_bounds brings the blocks' bounds up to date. A draft step with few
  * blocks: q27b_attn_prep, q27b_kv_bounds, q27b_select_blocks, q27b_attn_decode_blocks.
  * Their scratch lies in the workspace, of one sequence in the prefill buffer (at its fixed size; a smaller one makes for fewer
- * parts, or Q27B_UNSUPPORTED), over pages in the paged buffer: calls that can overlap on the GPU race on it, so keep those of
- * one device in one stream order. Float and cache pointers lie on 16-byte boundaries. Indices that the device finds out of
- * range are skipped and reported in the device status word (bit 1: page table, bit 2: path or list of blocks). */
+ * parts, or Q27B_UNSUPPORTED) or, for trees of up to four drafts, in the decode buffer; over pages in the paged buffer. Calls
+ * that can overlap on the GPU race on it, so keep those of one device in one stream order. Float and cache pointers lie on
+ * 16-byte boundaries. Indices that the device finds out of range are reported in the device status word (bit 1: page table,
+ * bit 2: path or list of blocks) and nothing is read or written there: a path's or list's entry is skipped, the rows of a
+ * page are skipped or, for trees of up to four drafts as in q27b_attn_decode_paged, stand for those of page 0. */
 
 /* Masks and depths of a tree of T = 1..64 drafts in which parent[t] is the draft before t (smaller than t) or -1 for a
  * child of the last accepted token: mask[t] has bit j set for j = t and every ancestor j of t, depth[t] (may be null)
@@ -446,15 +448,13 @@ int q27b_tree_plan(const int* parent, int T, uint64_t* mask, int* depth);
  * *pos0 + j for which bit j of mask[t] is set (its own only if bit t is; bits from T on are ignored); what the other rows
  * hold has no influence. Otherwise as q27b_attn_decode: GQA 6:1, softmax, o *= sigmoid(gate); a draft that sees nothing
  * gives 0. mask is device memory. Q * kq_scale, K, V and P are rounded to f16 for the tensor cores, sums are f32; the
- * output is therefore f16 (o: __half [T][nqh][256]) or, with xq != null, q8_1 as in q27b_attn_decode. Partials lie in
- * the prefill workspace. */
+ * output is therefore f16 (o: __half [T][nqh][256]) or, with xq != null, q8_1 as in q27b_attn_decode. */
 int q27b_attn_decode_tree(const float* qn, const float* qg, const void* kcache, const void* vcache, void* o, int8_t* xq,
                           float* xd, const int* pos0, const uint64_t* mask, int T, float kq_scale, int nqh, int nkvh,
                           int n_ctx, int q8, void* stream);
 /* The same for B sequences over the page pool: T drafts each at positions seq_len[b] - T + t (seq_len counts them),
  * mask [B][T]. max_seq_len: no seq_len[b] is larger (a longer one is cut there). Sequences with fewer drafts give the rows
- * they do not use a mask of 0 and name them in no other: what such rows hold does not matter. B * T <= 65535. Partials lie
- * in the paged workspace. */
+ * they do not use a mask of 0 and name them in no other: what such rows hold does not matter. B * T <= 65535. */
 int q27b_attn_decode_tree_paged(const float* qn, const float* qg, const void* kpool, const void* vpool,
                                 const int* page_table, const int* seq_len, const uint64_t* mask, void* o, int8_t* xq,
                                 float* xd, int B, int T, float kq_scale, int nqh, int nkvh, int n_pages, int max_pages,

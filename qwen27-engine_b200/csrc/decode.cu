@@ -173,7 +173,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
   const int g = lane >> 2, tg = lane & 3;
 
   // Local rows to attend, and this CTA's chunk [c0, c1) of them (multiples of TILE).
-  int n = pos0 + T - p.base_pos;
+  int n = pos0 + T - p.hold - p.base_pos;
   if (p.n_local >= 0) n = min(n, p.n_local);
   n = max(0, min(n, p.n_ctx));
   int chunk;
@@ -733,6 +733,46 @@ int noalloc_setup(int dev) {
 }
 
 }  // namespace
+
+int launch_prefix(DeviceCtx* ctx, const float* qn, const void* kcache, const void* vcache, const int* pos0, int T, float kq_scale,
+                  int nkvh, int n_ctx, bool q8, PrefixPartials* out, cudaStream_t s) {
+  float* part;
+  if (int rc = decode_ws(ctx, &part)) return rc;
+  CUtensorMap kv, ks, vv, vs;
+  if (int rc = get_tmaps(kcache, nkvh, n_ctx, q8, &kv, &ks)) return rc;
+  if (int rc = get_tmaps(vcache, nkvh, n_ctx, q8, &vv, &vs)) return rc;
+  DecodeParams p = {};
+  p.qn = qn; p.part = part; p.pos0 = pos0; p.status = ctx->status; p.T = T; p.nqh = nkvh * GQA; p.nkvh = nkvh; p.n_ctx = n_ctx;
+  p.nch = ctx->n_sm / nkvh; p.kq_scale = kq_scale; p.n_local = -1; p.hold = T;
+  *out = {part, p.nch, 0};
+  // (equal static shares: the same bits on every run)
+  return q8 ? launch_decode_ws(&kv, &ks, &vv, &vs, p, false, 1, s) : launch_decode_t<false, false>(&kv, &ks, &vv, &vs, p, 1, s);
+}
+
+int launch_prefix_paged(DeviceCtx* ctx, const float* qn, const void* kpool, const void* vpool, const int* page_table,
+                        const int* seq_len, int B, int T, float kq_scale, int nkvh, int n_pages, int max_pages, int max_seq_len,
+                        const char* who, PrefixPartials* out, cudaStream_t s) {
+  // A chunk a CTA: one for every SM while that is at most 1,024 positions (a sequence of 1,024: 9.4 us in chunks of 128 and 26.2
+  // in one of 1,024; eight of up to 1,024: 16.5 and 30.8), longer ones when there would be more than sixteen for an SM (16 of up
+  // to 16,384: 87 in chunks of 1,024, 96 of 1,792, 83 of 2,048, 134 of 4,096; 64 of up to 4,096: 131, 141, 137, 159). Four
+  // drafts each; only the longest possible lengths are known here.
+  const int64_t per_sm = ((int64_t)B * nkvh * max_seq_len + ctx->n_sm - 1) / ctx->n_sm;
+  int chunk = (int)std::max<int64_t>(std::min<int64_t>(1024, per_sm), std::min<int64_t>(4096, per_sm / 16));
+  chunk = std::max(128, (chunk + 63) / 64 * 64);
+  const int nch = (max_seq_len + chunk - 1) / chunk;
+  float* part;
+  if (int rc = paged_ws(ctx, (size_t)B * nkvh * nch * MAXR * PROW, &part, who)) return rc;
+  CUtensorMap kv, ks, vv, vs;
+  if (int rc = get_tmaps(kpool, nkvh, n_pages * Q27B_PAGE, true, &kv, &ks)) return rc;
+  if (int rc = get_tmaps(vpool, nkvh, n_pages * Q27B_PAGE, true, &vv, &vs)) return rc;
+  DecodeParams p = {};
+  p.qn = qn; p.part = part; p.status = ctx->status; p.T = T; p.nqh = nkvh * GQA; p.nkvh = nkvh; p.n_ctx = max_seq_len; p.nch = nch;
+  p.kq_scale = kq_scale; p.n_local = -1; p.hold = T; p.page_table = page_table; p.seq_len = seq_len; p.max_pages = max_pages;
+  p.n_pages = n_pages; p.chunk_len = chunk;
+  *out = {part, nch, chunk};
+  const bool spread = (int64_t)nch * nkvh * B <= ctx->n_sm;
+  return launch_decode_ws(&kv, &ks, &vv, &vs, p, true, B, s, spread ? WsGroups::SPREAD : WsGroups::PAIRED);
+}
 
 int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const DecodeParams& p, int nseq, cudaStream_t s) {
   static bool attr[64] = {};

@@ -14,6 +14,7 @@ struct DecodeParams {
   float kq_scale;
   int base_pos;      // global position of local cache row 0
   int n_local;       // local rows to attend; < 0: all rows up to *pos0 + T
+  int hold;          // rows at the end that are left out: T for the prefix alone (launch_prefix)
   // paged / batched variant: grid (chunks, nkvh, B), fixed chunk length, rows through the page table
   const int* page_table;  // [B][max_pages]
   const int* seq_len;     // [B], counts the T new tokens
@@ -64,6 +65,18 @@ int launch_decode_wt(const CUtensorMap* kv, const CUtensorMap* ks, const CUtenso
 int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                      const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups);
 int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const DecodeParams& p, int nseq, cudaStream_t s);
+// The attention of T = 1..4 tokens to the rows before them alone, by the kernels of a decode call (q8_0: the warp-specialised one;
+// f16: decode.cu); partials [sequence][KV head][chunk][24][258].
+struct PrefixPartials {
+  const float* part;
+  int nch;        // chunks of a KV head
+  int chunk_len;  // their length over pages; 0: as filled_chunks says
+};
+int launch_prefix(DeviceCtx* ctx, const float* qn, const void* kcache, const void* vcache, const int* pos0, int T, float kq_scale,
+                  int nkvh, int n_ctx, bool q8, PrefixPartials* out, cudaStream_t s);
+int launch_prefix_paged(DeviceCtx* ctx, const float* qn, const void* kpool, const void* vpool, const int* page_table,
+                        const int* seq_len, int B, int T, float kq_scale, int nkvh, int n_pages, int max_pages, int max_seq_len,
+                        const char* who, PrefixPartials* out, cudaStream_t s);
 // Opts the kernels of decode_ws.cu into their shared-memory size on the current device.
 int decode_ws_setup();
 

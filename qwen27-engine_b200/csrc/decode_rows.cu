@@ -4,8 +4,8 @@
 // y = sigmoid(gate) * sum_p P_p v_p with P the softmax of kq_scale * q.k over the visible rows p, in f32; 0 where a row
 // sees nothing. Rows that are not visible are not read, whatever they hold.
 //
-// The split kernels leave the partials (m, l, O) of a row for every share of its positions; the kernel here merges them. Trees:
-// decode_tree.cu. Lists of blocks: the split-K kernels of decode_ws.cu (q8_0) and decode.cu (f16), a chunk of a list a CTA,
+// The split kernels leave the partials (m, l, O) of a row for every part of its positions; the kernels here merge them. Trees:
+// decode_tree.cu, or for up to four drafts the kernels of q27b_attn_decode over the prefix. Lists of blocks: the split-K kernels of decode_ws.cu (q8_0) and decode.cu (f16), a chunk of a list a CTA,
 // every (token, KV head) for itself.
 #include "cache_ref.h"
 #include "decode_params.h"
@@ -13,6 +13,29 @@
 
 namespace q27b {
 namespace {
+
+// Dims 4 c .. 4 c + 3 of a row (c = 0..63, two whole warps): A / L times the gate, as f16 or q8_1.
+__device__ __forceinline__ void write_row(const RowsParams& p, size_t row, int c, const float4& A, float L, const float4& g) {
+  const float inv = L == 0.f ? 0.f : 1.0f / L;
+  float out[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
+  const float gv[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) out[i] *= 1.0f / (1.0f + expf(-gv[i]));
+  if (!p.xq) {
+    *(uint2*)((__half*)p.o + row * AD + 4 * c) = make_uint2(pack_h2(out[0], out[1]), pack_h2(out[2], out[3]));
+    return;
+  }
+  // q8_1 of 32 dims = eight lanes, as the merge of attn_decode writes it
+  float amax = fmaxf(fmaxf(fabsf(out[0]), fabsf(out[1])), fmaxf(fabsf(out[2]), fabsf(out[3])));
+#pragma unroll
+  for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float d = __fdiv_rn(amax, 127.0f);
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) w |= (uint32_t)((amax == 0.0f ? 0 : (int)roundf(__fdiv_rn(out[i], d))) & 0xFF) << (8 * i);
+  *(uint32_t*)(p.xq + row * AD + 4 * c) = w;
+  if ((c & 7) == 0) p.xd[(row * AD + 4 * c) / 32] = __half2float(__float2half_rn(d));
+}
 
 // Merges the partials of a row, applies the gate and writes f16, or q8_1; a row without a visible position is 0. 64 threads to
 // a row, four dims each, or GROUPS times as many that take every GROUPS-th partial; the first ten of each are requested before the
@@ -109,25 +132,96 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p, int
     }
   }
   if (!mine) return;
-  const float inv = L == 0.f ? 0.f : 1.0f / L;
-  float out[4] = {A.x * inv, A.y * inv, A.z * inv, A.w * inv};
-  const float gv[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-  for (int i = 0; i < 4; i++) out[i] *= 1.0f / (1.0f + expf(-gv[i]));
-  if (!p.xq) {
-    *(uint2*)((__half*)p.o + row * AD + 4 * c) = make_uint2(pack_h2(out[0], out[1]), pack_h2(out[2], out[3]));
-    return;
+  write_row(p, row, c, A, L, g);
+}
+
+// Up to four drafts: the partials of the prefix, and the drafts themselves, merged. One CTA a row, four groups of 64 threads, four
+// dims a thread; group j scores draft j (if the row sees it) and takes its V row as a partial (score, 1, v), in f32 and before the
+// partials are there; then every fourth partial.
+template <int PRE, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams p, const PrefixPartials pre) {
+  __shared__ float4 sa[3][64];
+  __shared__ float sl[4], sm[8], sd[8];
+  const size_t row = blockIdx.x;
+  const int tid = threadIdx.x, grp = tid >> 6, c = tid & 63, T = p.c.T, nqh = p.c.nkvh * GQA;
+  const int b = (int)(row / ((size_t)T * nqh)), t = (int)(row / nqh % T), h = (int)(row % nqh), kh = h / GQA;
+  const int first = first_pos(p.c, b), n = max(0, min(first, p.c.n_ctx));  // drafts, prefix
+  const float4 g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c), q = *(const float4*)(p.qn + row * AD + 4 * c);
+  const int64_t at = grp < T && ((p.mask[(size_t)b * T + t] >> grp) & 1) ? cache_row(p.c, b, kh, first + grp) : -1;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  float s = 0.f;
+  if (at >= 0) {
+    auto four = [&](const void* cache) {
+      const uint8_t* base = (const uint8_t*)cache;
+      if (!p.c.q8) {
+        const uint2 w = *(const uint2*)(base + at * 2 * AD + 8 * c);
+        const float2 lo = __half22float2(u32_as_h2(w.x)), hi = __half22float2(u32_as_h2(w.y));
+        return make_float4(lo.x, lo.y, hi.x, hi.y);
+      }
+      const uint32_t w = *(const uint32_t*)(base + at * AD + 4 * c);
+      const float d = __half2float(*(const __half*)(base + cache_rows(p.c) * AD + at * 16 + (c >> 3) * 2));
+      return make_float4((float)(int8_t)w * d, (float)(int8_t)(w >> 8) * d, (float)(int8_t)(w >> 16) * d, (float)(int8_t)(w >> 24) * d);
+    };
+    const float4 k = four(p.kcache);
+    v = four(p.vcache);
+    s = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
   }
-  // q8_1 of 32 dims = eight lanes, as the merge of attn_decode writes it
-  float amax = fmaxf(fmaxf(fabsf(out[0]), fabsf(out[1])), fmaxf(fabsf(out[2]), fabsf(out[3])));
 #pragma unroll
-  for (int o = 1; o <= 4; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float d = __fdiv_rn(amax, 127.0f);
-  uint32_t w = 0;
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((tid & 31) == 0) sd[tid >> 5] = at >= 0 ? s * p.kq_scale : M_INIT / 2;
+  int np = pre.chunk_len ? (n + pre.chunk_len - 1) / pre.chunk_len : n > 0 ? filled_chunks(n, pre.nch) : 0;
+  const float* po = pre.part + (((size_t)b * p.c.nkvh + kh) * pre.nch * MAXR + t * GQA + h % GQA) * PROW;  // chunks MAXR rows apart
+  pdl_wait();
+  pdl_trigger();
+  float2 x[PRE][2], ml[PRE];  // every fourth partial, PRE at a time
+  auto fetch = [&](int z0) {
 #pragma unroll
-  for (int i = 0; i < 4; i++) w |= (uint32_t)((amax == 0.0f ? 0 : (int)roundf(__fdiv_rn(out[i], d))) & 0xFF) << (8 * i);
-  *(uint32_t*)(p.xq + row * AD + 4 * c) = w;
-  if ((c & 7) == 0) p.xd[(row * AD + 4 * c) / 32] = __half2float(__float2half_rn(d));
+    for (int i = 0; i < PRE; i++)
+      if (z0 + 4 * i < np) {
+        const float* r = po + (size_t)(z0 + 4 * i) * MAXR * PROW;
+        ml[i] = *(const float2*)r;
+        x[i][0] = *(const float2*)(r + 2 + 4 * c);
+        x[i][1] = *(const float2*)(r + 4 + 4 * c);
+      }
+  };
+  fetch(grp);
+  float M = M_INIT;
+  for (int z = tid; z < np; z += 256) M = fmaxf(M, po[(size_t)z * MAXR * PROW]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if ((tid & 31) == 0) sm[tid >> 5] = M;
+  __syncthreads();
+  s = sd[2 * grp] + sd[2 * grp + 1];
+#pragma unroll
+  for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
+#pragma unroll
+  for (int j = 0; j < 4; j++) M = fmaxf(M, sd[2 * j] + sd[2 * j + 1]);
+  float L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float m, float l, float ax, float ay, float az, float aw) {
+    if (l == 0.f) return;  // holds nothing
+    const float f = ex2((m - M) * LOG2E);
+    L += l * f;
+    A.x += ax * f, A.y += ay * f, A.z += az * f, A.w += aw * f;
+  };
+  if (at >= 0) add(s, 1.f, v.x, v.y, v.z, v.w);
+  for (int z0 = grp; z0 < np; z0 += 4 * PRE) {
+    if (z0 > grp) fetch(z0);
+#pragma unroll
+    for (int i = 0; i < PRE; i++)
+      if (z0 + 4 * i < np) add(ml[i].x, ml[i].y, x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y);
+  }
+  if (grp > 0) sa[grp - 1][c] = A;
+  if (c == 0) sl[grp] = L;
+  __syncthreads();
+  if (grp > 0) return;
+#pragma unroll
+  for (int k = 0; k < 3; k++) {
+    const float4 y = sa[k][c];
+    A.x += y.x, A.y += y.y, A.z += y.z, A.w += y.w;
+    L += sl[k + 1];
+  }
+  write_row(p, row, c, A, L, g);
 }
 
 int launch_rows_merge(const RowsParams& p, int64_t rows, int n_sm, cudaStream_t s) {
@@ -214,6 +308,27 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
 }
 
 int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
+  const CacheRef& c = p.c;
+  if (c.T <= Q27B_MAX_T && c.nkvh <= ctx->n_sm && (c.q8 || (int64_t)c.nkvh * c.n_ctx <= 32768)) {
+    // Up to four drafts are 24 rows of a KV head. The decode kernels, made for those, take the prefix, and the merge the drafts:
+    // four behind 1,000 positions 9.4 us against 10.6 with the 128-row tiles of decode_tree.cu, behind 150,000 75 against 98, a
+    // single one 59 against 89; four each behind 16 sequences of up to 16,384 87 against 109, of 2,048 to 4,096 49 against 54, of
+    // 64 to 4,096 48 against 44. An f16 cache has nothing to convert there and is bound by its reads earlier: four behind 8,000
+    // 18.4 against 19.4, behind 16,000 27 against 25, behind 150,000 129 against 106.
+    PrefixPartials pre;
+    if (c.page_table) {
+      if (int rc = launch_prefix_paged(ctx, p.qn, p.kcache, p.vcache, c.page_table, c.seq_len, c.B, c.T, p.kq_scale, c.nkvh, c.n_pages,
+                                       c.max_pages, c.n_ctx, who, &pre, s))
+        return rc;
+    } else if (int rc = launch_prefix(ctx, p.qn, p.kcache, p.vcache, c.pos0, c.T, p.kq_scale, c.nkvh, c.n_ctx, c.q8, &pre, s)) {
+      return rc;
+    }
+    const dim3 grid((unsigned)(c.B * c.T * c.nkvh * GQA));
+    // Many rows: fewer partials in flight for each, more rows on an SM (16 sequences of four drafts 48 us and 56).
+    if ((int64_t)grid.x >= 4 * (int64_t)ctx->n_sm) Q27B_CK(launch_step(draft_merge_kernel<4, 5>, grid, dim3(256), 0, s, p, pre));
+    else Q27B_CK(launch_step(draft_merge_kernel<10, 2>, grid, dim3(256), 0, s, p, pre));
+    return Q27B_OK;
+  }
   const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, units = (int64_t)p.c.B * p.c.nkvh * tree_row_tiles(p.c.T);
   const bool paged = p.c.page_table != nullptr;
   const int64_t head = paged ? (2 * (p.c.B + 1) + 3) / 4 * 4 : 0;  // the plan, in floats

@@ -220,7 +220,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   // from one by one when their own tiles are done (the SMs do not stream at equal rates: with equal
   // static shares the slowest CTA of a 150k-position call ends 5 us after the median one). A CTA
   // folds whatever tiles it gets into one partial: the log-sum-exp merge does not care which.
-  int n = pos0 + T - p.base_pos;
+  int n = pos0 + T - p.hold - p.base_pos;
   if (p.n_local >= 0) n = min(n, p.n_local);
   n = max(0, min(n, p.n_ctx));
   int t_first, n_static, n_end, pool0, ntiles_all;

@@ -423,3 +423,63 @@ def test_other_launch_modes(q27, mode):
                        env=dict(os.environ, Q27_PDL=mode), capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-1000:]
     assert " passed" in r.stdout
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("nkvh", [1, 4])
+@pytest.mark.parametrize("T", [1, 2, 3, 4])
+def test_few_drafts(q27, T, nkvh, q8):
+    """Up to four drafts of one sequence, with a prefix of nothing, up to and past a tile, and of many parts; in a cache that ends
+    there and in a long one (an f16 cache of more than 32,768 rows takes the kernel of wide trees)."""
+    for n in (T, T + 1, T + 63, T + 64, T + 65, 700, 9001):
+        for n_ctx in (n, 40000):
+            st = H.Store([n], T, nkvh, False, q8, seed=n, n_ctx=n_ctx)
+            kc, vc = st.new(), st.new()
+            st.fill(kc, H.gen(n))
+            st.fill(vc, H.gen(n + 1))
+            masks = H.random_masks(1, T, seed=n)
+            if n == 700:
+                masks[0][T - 1] = 0  # sees the prefix alone
+            qn, qg = H.queries(st, 3)
+            o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+            H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 4])
+@pytest.mark.parametrize("lens", [[4], [5, 300, 128, 132], [1000] * 9 + [64] * 5, [100, 9000], [4100, 700] * 20])
+def test_few_drafts_of_a_batch(q27, lens, T):
+    st = H.Store(lens, T, 2, True, True, seed=T)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    masks = H.random_masks(st.B, T, seed=T)
+    qn, qg = H.queries(st, 3)
+    o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+    H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+    assert torch.equal(o, H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks)))
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("paged,q8", [(False, True), (False, False), (True, True)])
+def test_few_drafts_poisoned_rows_and_runaway_scores(q27, paged, q8):
+    """Drafts that nobody sees are NaN, beside the last rows of the prefix in their tile; the scores of those that are seen are
+    far above or below those of the prefix (tolerance as for scores that run away)."""
+    T, lens = 4, [333, 68, 4] if paged else [333]
+    st = H.Store(lens, T, 2, paged, q8, seed=4)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    qn, qg = H.queries(st, 3)
+    for b, n in enumerate(lens):
+        for h in range(2):
+            st.poison(kc, b, h, [n - 3, n - 1])
+            st.poison(vc, b, h, [n - 3, n - 1])
+            st.write(kc, b, h, [n - 4, n - 2], 40.0 * torch.cat([qn[b, 0, 6 * h][None], -qn[b, 2, 6 * h][None]]))
+    masks = [[0b0001, 0b0001, 0b0101, 0b0100] for _ in lens]
+    o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+    ref = H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks))
+    ds = ref[2] * (2.0 ** -10 + 2.0 ** -16)
+    tol = ref[1] * (torch.expm1(2 * ds) + 2.0 ** -10)[..., None] + (ref[3] * 2.0 ** -25)[..., None] + ref[0].abs() * 2.0 ** -11 + 2.0 ** -25
+    assert ((o.view(ref[0].shape).double() - ref[0]).abs() <= tol).all()
+    assert q27.device_status() == 0
