@@ -38,12 +38,12 @@ __device__ __forceinline__ void write_row(const RowsParams& p, size_t row, int c
 }
 
 // Merges the partials of a row, applies the gate and writes f16, or q8_1; a row without a visible position is 0. 64 threads to
-// a row, four dims each, or GROUPS times as many that take every GROUPS-th partial; the first ten of each are requested before the
-// maxima are known. Many rows have few partials each (a batch): four rows to a CTA of 256 threads then.
-constexpr int MERGE_PRE = 10;
-
-template <int GROUPS>
-__global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p, int64_t rows) {
+// a row, four dims each, or four times as many that take every fourth partial; PRE partials of a thread are requested at a time, the
+// first before the maxima are known. 72 rows of 148 partials: PRE = 10 and two CTAs on an SM 18.4 us a call, 6 and three 20.1;
+// 384 rows of 49, which fill the SMs more than once with two CTAs: 29.0 and 26.4. Many rows have few partials each (a batch): a
+// CTA takes four rows then (6,144 rows of a few partials: 151.8 and 134.3 us a call, a CTA for every row 224).
+template <int GROUPS, int PRE, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams p, int64_t rows) {
   constexpr int ROWS = 4 / GROUPS;  // of a CTA
   __shared__ float4 sa[GROUPS > 1 ? GROUPS - 1 : 1][64];
   __shared__ float sl[4], sm[8];
@@ -86,14 +86,17 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p, int
   }
   const float2* ml = p.part_ml + first;
   const float* po = p.part_o + first * AD + 4 * c;
-  float4 pre[MERGE_PRE];
-  float2 pml[MERGE_PRE];
+  float4 x[PRE];  // every GROUPS-th partial, PRE at a time
+  float2 xml[PRE];
+  auto fetch = [&](int z0) {
 #pragma unroll
-  for (int i = 0; i < MERGE_PRE; i++)
-    if (grp + GROUPS * i < np) {
-      pre[i] = *(const float4*)(po + (size_t)(grp + GROUPS * i) * step * AD);
-      pml[i] = ml[(size_t)(grp + GROUPS * i) * step];
-    }
+    for (int i = 0; i < PRE; i++)
+      if (z0 + GROUPS * i < np) {
+        x[i] = *(const float4*)(po + (size_t)(z0 + GROUPS * i) * step * AD);
+        xml[i] = ml[(size_t)(z0 + GROUPS * i) * step];
+      }
+  };
+  fetch(grp);
   float M = M_INIT;
   for (int z = GROUPS > 1 ? tid : c; z < np; z += 64 * GROUPS) M = fmaxf(M, ml[(size_t)z * step].x);
 #pragma unroll
@@ -114,11 +117,12 @@ __global__ void __launch_bounds__(256) rows_merge_kernel(const RowsParams p, int
     L += v.y * f;
     A.x += x.x * f, A.y += x.y * f, A.z += x.z * f, A.w += x.w * f;
   };
+  for (int z0 = grp; z0 < np; z0 += GROUPS * PRE) {
+    if (z0 > grp) fetch(z0);
 #pragma unroll
-  for (int i = 0; i < MERGE_PRE; i++)
-    if (grp + GROUPS * i < np) add(pml[i], pre[i]);
-#pragma unroll 4
-  for (int z = grp + GROUPS * MERGE_PRE; z < np; z += GROUPS) add(ml[(size_t)z * step], *(const float4*)(po + (size_t)z * step * AD));
+    for (int i = 0; i < PRE; i++)
+      if (z0 + GROUPS * i < np) add(xml[i], x[i]);
+  }
   if (GROUPS > 1) {
     if (grp > 0) sa[grp - 1][c] = A;
     if (c == 0) sl[grp] = L;
@@ -225,8 +229,9 @@ __global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams
 }
 
 int launch_rows_merge(const RowsParams& p, int64_t rows, int n_sm, cudaStream_t s) {
-  if (rows >= 8 * (int64_t)n_sm) Q27B_CK(launch_step(rows_merge_kernel<1>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, p, rows));
-  else Q27B_CK(launch_step(rows_merge_kernel<4>, dim3((unsigned)rows), dim3(256), 0, s, p, rows));
+  const bool split = rows < 8 * (int64_t)n_sm;  // a row's partials among the groups of a CTA
+  auto* k = !split ? rows_merge_kernel<1, 6, 3> : rows > 2 * (int64_t)n_sm ? rows_merge_kernel<4, 6, 3> : rows_merge_kernel<4, 10, 2>;
+  Q27B_CK(launch_step(k, dim3((unsigned)(split ? rows : (rows + 3) / 4)), dim3(256), 0, s, p, rows));
   return Q27B_OK;
 }
 

@@ -11,7 +11,7 @@ namespace {
 // ---------------------------------------------------------------- commit
 // Row first + i <- row first + path[i] for i < count, K and V, every head. A CTA owns one (head, K or V, sequence): it
 // holds all moved rows in registers (up to 64 rows of 272 or 512 bytes in 256 threads) before it writes the first, so a
-// path may name rows in any order. Launch and latency bound: 64 rows of 4 heads are 0.3 MB.
+// path may name rows in any order. Launch and latency bound: 16 drafts of one sequence 3.3 us a call, 64 of each of 64 sequences 4.1.
 constexpr int COMMIT_WARPS = 8, COMMIT_ROWS = MAX_TREE_T / COMMIT_WARPS;
 
 __global__ void __launch_bounds__(32 * COMMIT_WARPS) commit_kernel(const CacheRef c, void* kcache, void* vcache, const int* path,
@@ -247,7 +247,9 @@ __device__ __forceinline__ int blocks_of(const CacheRef& c, int b, int t) {
 // of two f16 values, off by at most 2^-22 of itself or 2^-25. Four accumulators: q+ hi and q- lo, with the larger parts and with
 // the smaller ones, 16 MMAs each. With A = sum |q| max(|lo|, |hi|) (a fifth one, of |q| + 2^-6), and 17 addends of
 // an MMA each cut at 2^-23 of the largest, the error is below 16 * 18 * 2^-23 A + 2^-22 A < 2^-14.7 A; 2^-14 A is what is
-// passed on. Bound by reading the bounds once they fill the SMs.
+// passed on. 32 sequences of up to 131,072 positions, two tokens: 45 us for 147 MB of bounds, between the latency of their loads
+// (a quarter of the issue slots and of the tensor pipe is used; more warps would need the registers that hold loads in flight) and
+// memory; one token behind 150,000 positions: one trip to memory, 4 us.
 constexpr int SCORE_WARPS = 4, SCORE_GROUP = 16 * SCORE_WARPS, Q_STRIDE = 2 * AD + 64;  // bytes between staged query rows: 16-byte reads without conflicts
 enum { QP_HI, QM_HI, QP_LO, QM_LO, QABS, Q_PARTS };
 constexpr int Q_TOKEN = Q_PARTS * 8 * Q_STRIDE;  // bytes of a staged token
@@ -503,7 +505,9 @@ __device__ K nth_largest(F key, int n, int want, int few, SelShared& sh, K* mask
 // that holds the want-th largest s: want blocks or more have a score of at least t0 - E, so a block of s + e < t0 - E is
 // out; the scores of the blocks with s <= t1 are at most t1 + E, and fewer than want have a larger s, so a block of s - e > t1 + E
 // is in. The blocks between are scored again in 64 bits, a warp each, and the best of them fill up the list; of equal ones the
-// lower. Where something is not finite, or everything alike, these are all blocks. Bound by the latency of a dozen barriers.
+// lower. Where something is not finite, or everything alike, these are all blocks. Bound by the latency of a dozen barriers and of
+// the trips to memory (scores, then the bounds of the open blocks): about 8 of the 13 us of a call on 2,344 blocks of four heads,
+// k = 128. Counting by the bits of the scores, three turns instead of one, took 2.6 us longer.
 __global__ void __launch_bounds__(SEL_THREADS, 2) select_kernel(const SelectParams p) {
   extern __shared__ uint64_t dyn[];  // [max_blocks] (score, error), then the 64-bit keys of the open blocks; then their numbers
   __shared__ SelShared sh;
