@@ -139,50 +139,61 @@ __global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams 
   write_row(p, row, c, A, L, g);
 }
 
-// Up to four drafts: the partials of the prefix, and the drafts themselves, merged. One CTA a row, four groups of 64 threads, four
-// dims a thread; group j scores draft j (if the row sees it) and takes its V row as a partial (score, 1, v), in f32 and before the
-// partials are there; then every fourth partial.
-template <int PRE, int CTAS>
-__global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams p, const PrefixPartials pre) {
-  __shared__ float4 sa[3][64];
-  __shared__ float sl[4], sm[8], sd[8];
-  const size_t row = blockIdx.x;
-  const int tid = threadIdx.x, grp = tid >> 6, c = tid & 63, T = p.c.T, nqh = p.c.nkvh * GQA;
+// Up to four drafts: the partials of the prefix, and the drafts themselves, merged. 64 threads to a row, four dims each, or four
+// times as many (GROUPS) that share the drafts and the partials out. A draft that the row sees is scored, and its V row taken as a
+// partial (score, 1, v), in f32 and before the partials are there. 24 rows of 148 partials: 25.1 us a call with groups and ten in
+// flight, 27.5 with six and three CTAs on an SM, 38 without groups; 384 rows of up to 32 76.2, 74.0 and 77; 6,144 rows of up to four 157,
+// 133 and 99.9 (without groups, four in flight).
+template <int GROUPS, int PRE, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams p, const PrefixPartials pre, int64_t rows) {
+  constexpr int ROWS = 4 / GROUPS, DRAFTS = 4 / GROUPS;  // rows of a CTA, drafts of a thread
+  __shared__ float4 sa[GROUPS > 1 ? GROUPS - 1 : 1][64];
+  __shared__ float sl[4], sm[8], sd[8][DRAFTS];
+  const int tid = threadIdx.x, warp = tid >> 5, c = tid & 63, grp = GROUPS > 1 ? tid >> 6 : 0;
+  const size_t row = min((int64_t)blockIdx.x * ROWS + (GROUPS > 1 ? 0 : tid >> 6), rows - 1);  // rows beyond the last do its work again
+  const int T = p.c.T, nqh = p.c.nkvh * GQA;
   const int b = (int)(row / ((size_t)T * nqh)), t = (int)(row / nqh % T), h = (int)(row % nqh), kh = h / GQA;
   const int first = first_pos(p.c, b), n = max(0, min(first, p.c.n_ctx));  // drafts, prefix
   const float4 g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c), q = *(const float4*)(p.qn + row * AD + 4 * c);
-  const int64_t at = grp < T && ((p.mask[(size_t)b * T + t] >> grp) & 1) ? cache_row(p.c, b, kh, first + grp) : -1;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  float s = 0.f;
-  if (at >= 0) {
-    auto four = [&](const void* cache) {
-      const uint8_t* base = (const uint8_t*)cache;
-      if (!p.c.q8) {
-        const uint2 w = *(const uint2*)(base + at * 2 * AD + 8 * c);
-        const float2 lo = __half22float2(u32_as_h2(w.x)), hi = __half22float2(u32_as_h2(w.y));
-        return make_float4(lo.x, lo.y, hi.x, hi.y);
-      }
-      const uint32_t w = *(const uint32_t*)(base + at * AD + 4 * c);
-      const float d = __half2float(*(const __half*)(base + cache_rows(p.c) * AD + at * 16 + (c >> 3) * 2));
-      return make_float4((float)(int8_t)w * d, (float)(int8_t)(w >> 8) * d, (float)(int8_t)(w >> 16) * d, (float)(int8_t)(w >> 24) * d);
-    };
-    const float4 k = four(p.kcache);
-    v = four(p.vcache);
-    s = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+  const uint64_t mask = p.mask[(size_t)b * T + t];
+  auto four = [&](const void* cache, int64_t at) {
+    const uint8_t* base = (const uint8_t*)cache;
+    if (!p.c.q8) {
+      const uint2 w = *(const uint2*)(base + at * 2 * AD + 8 * c);
+      const float2 lo = __half22float2(u32_as_h2(w.x)), hi = __half22float2(u32_as_h2(w.y));
+      return make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+    const uint32_t w = *(const uint32_t*)(base + at * AD + 4 * c);
+    const float d = __half2float(*(const __half*)(base + cache_rows(p.c) * AD + at * 16 + (c >> 3) * 2));
+    return make_float4((float)(int8_t)w * d, (float)(int8_t)(w >> 8) * d, (float)(int8_t)(w >> 16) * d, (float)(int8_t)(w >> 24) * d);
+  };
+  float4 k[DRAFTS], v[DRAFTS];
+  bool seen[DRAFTS];
+#pragma unroll
+  for (int d = 0; d < DRAFTS; d++) {
+    const int j = grp + d;
+    const int64_t at = j < T && ((mask >> j) & 1) ? cache_row(p.c, b, kh, first + j) : -1;
+    k[d] = v[d] = make_float4(0.f, 0.f, 0.f, 0.f);
+    seen[d] = at >= 0;
+    if (seen[d]) k[d] = four(p.kcache, at), v[d] = four(p.vcache, at);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((tid & 31) == 0) sd[tid >> 5] = at >= 0 ? s * p.kq_scale : M_INIT / 2;
-  int np = pre.chunk_len ? (n + pre.chunk_len - 1) / pre.chunk_len : n > 0 ? filled_chunks(n, pre.nch) : 0;
+  for (int d = 0; d < DRAFTS; d++) {
+    float s = q.x * k[d].x + q.y * k[d].y + q.z * k[d].z + q.w * k[d].w;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if ((tid & 31) == 0) sd[warp][d] = seen[d] ? s * p.kq_scale : M_INIT / 2;
+  }
+  const int np = pre.chunk_len ? (n + pre.chunk_len - 1) / pre.chunk_len : n > 0 ? filled_chunks(n, pre.nch) : 0;
   const float* po = pre.part + (((size_t)b * p.c.nkvh + kh) * pre.nch * MAXR + t * GQA + h % GQA) * PROW;  // chunks MAXR rows apart
   pdl_wait();
   pdl_trigger();
-  float2 x[PRE][2], ml[PRE];  // every fourth partial, PRE at a time
+  float2 x[PRE][2], ml[PRE];  // every GROUPS-th partial, PRE at a time
   auto fetch = [&](int z0) {
 #pragma unroll
     for (int i = 0; i < PRE; i++)
-      if (z0 + 4 * i < np) {
-        const float* r = po + (size_t)(z0 + 4 * i) * MAXR * PROW;
+      if (z0 + GROUPS * i < np) {
+        const float* r = po + (size_t)(z0 + GROUPS * i) * MAXR * PROW;
         ml[i] = *(const float2*)r;
         x[i][0] = *(const float2*)(r + 2 + 4 * c);
         x[i][1] = *(const float2*)(r + 4 + 4 * c);
@@ -190,16 +201,22 @@ __global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams
   };
   fetch(grp);
   float M = M_INIT;
-  for (int z = tid; z < np; z += 256) M = fmaxf(M, po[(size_t)z * MAXR * PROW]);
+  for (int z = GROUPS > 1 ? tid : c; z < np; z += 64 * GROUPS) M = fmaxf(M, po[(size_t)z * MAXR * PROW]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  if ((tid & 31) == 0) sm[tid >> 5] = M;
+  if ((tid & 31) == 0) sm[warp] = M;
   __syncthreads();
-  s = sd[2 * grp] + sd[2 * grp + 1];
+  const int pair = warp & ~1;  // the two warps of this group
+  if (GROUPS > 1) {
 #pragma unroll
-  for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
+    for (int w = 0; w < 8; w++) M = fmaxf(M, sm[w]);
 #pragma unroll
-  for (int j = 0; j < 4; j++) M = fmaxf(M, sd[2 * j] + sd[2 * j + 1]);
+    for (int w = 0; w < 8; w += 2) M = fmaxf(M, sd[w][0] + sd[w + 1][0]);
+  } else {
+    M = fmaxf(sm[pair], sm[pair + 1]);
+#pragma unroll
+    for (int d = 0; d < DRAFTS; d++) M = fmaxf(M, sd[pair][d] + sd[pair + 1][d]);
+  }
   float L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
   auto add = [&](float m, float l, float ax, float ay, float az, float aw) {
@@ -208,22 +225,26 @@ __global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams
     L += l * f;
     A.x += ax * f, A.y += ay * f, A.z += az * f, A.w += aw * f;
   };
-  if (at >= 0) add(s, 1.f, v.x, v.y, v.z, v.w);
-  for (int z0 = grp; z0 < np; z0 += 4 * PRE) {
+#pragma unroll
+  for (int d = 0; d < DRAFTS; d++)
+    if (seen[d]) add(sd[pair][d] + sd[pair + 1][d], 1.f, v[d].x, v[d].y, v[d].z, v[d].w);
+  for (int z0 = grp; z0 < np; z0 += GROUPS * PRE) {
     if (z0 > grp) fetch(z0);
 #pragma unroll
     for (int i = 0; i < PRE; i++)
-      if (z0 + 4 * i < np) add(ml[i].x, ml[i].y, x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y);
+      if (z0 + GROUPS * i < np) add(ml[i].x, ml[i].y, x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y);
   }
-  if (grp > 0) sa[grp - 1][c] = A;
-  if (c == 0) sl[grp] = L;
-  __syncthreads();
-  if (grp > 0) return;
+  if (GROUPS > 1) {
+    if (grp > 0) sa[grp - 1][c] = A;
+    if (c == 0) sl[grp] = L;
+    __syncthreads();
+    if (grp > 0) return;
 #pragma unroll
-  for (int k = 0; k < 3; k++) {
-    const float4 y = sa[k][c];
-    A.x += y.x, A.y += y.y, A.z += y.z, A.w += y.w;
-    L += sl[k + 1];
+    for (int i = 0; i < GROUPS - 1; i++) {
+      const float4 y = sa[i][c];
+      A.x += y.x, A.y += y.y, A.z += y.z, A.w += y.w;
+      L += sl[i + 1];
+    }
   }
   write_row(p, row, c, A, L, g);
 }
@@ -316,9 +337,8 @@ int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   const CacheRef& c = p.c;
   if (c.T <= Q27B_MAX_T && c.nkvh <= ctx->n_sm && (c.q8 || (int64_t)c.nkvh * c.n_ctx <= 32768)) {
     // Up to four drafts are 24 rows of a KV head. The decode kernels, made for those, take the prefix, and the merge the drafts:
-    // four behind 1,000 positions 9.4 us against 10.6 with the 128-row tiles of decode_tree.cu, behind 150,000 75 against 98, a
-    // single one 59 against 89; four each behind 16 sequences of up to 16,384 87 against 109, of 2,048 to 4,096 49 against 54, of
-    // 64 to 4,096 48 against 44. An f16 cache has nothing to convert there and is bound by its reads earlier: four behind 8,000
+    // four behind 1,000 positions 9.2 us against 10.6 with the 128-row tiles of decode_tree.cu, behind 150,000 74 against 98, a
+    // single one 58 against 89; four each behind 16 sequences of up to 16,384 78 against 109, of 64 to 4,096 38 against 44. An f16 cache has nothing to convert there and is bound by its reads earlier: four behind 8,000
     // 18.4 against 19.4, behind 16,000 27 against 25, behind 150,000 129 against 106.
     PrefixPartials pre;
     if (c.page_table) {
@@ -328,10 +348,10 @@ int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
     } else if (int rc = launch_prefix(ctx, p.qn, p.kcache, p.vcache, c.pos0, c.T, p.kq_scale, c.nkvh, c.n_ctx, c.q8, &pre, s)) {
       return rc;
     }
-    const dim3 grid((unsigned)(c.B * c.T * c.nkvh * GQA));
-    // Many rows: fewer partials in flight for each, more rows on an SM (16 sequences of four drafts 48 us and 56).
-    if ((int64_t)grid.x >= 4 * (int64_t)ctx->n_sm) Q27B_CK(launch_step(draft_merge_kernel<4, 5>, grid, dim3(256), 0, s, p, pre));
-    else Q27B_CK(launch_step(draft_merge_kernel<10, 2>, grid, dim3(256), 0, s, p, pre));
+    const int64_t rows = (int64_t)c.B * c.T * c.nkvh * GQA;
+    const bool split = rows <= 4 * (int64_t)ctx->n_sm;
+    auto* k = !split ? draft_merge_kernel<1, 4, 3> : rows > 2 * (int64_t)ctx->n_sm ? draft_merge_kernel<4, 6, 3> : draft_merge_kernel<4, 10, 2>;
+    Q27B_CK(launch_step(k, dim3((unsigned)(split ? rows : (rows + 3) / 4)), dim3(256), 0, s, p, pre, rows));
     return Q27B_OK;
   }
   const int64_t rows = (int64_t)p.c.B * p.c.T * p.c.nkvh * GQA, units = (int64_t)p.c.B * p.c.nkvh * tree_row_tiles(p.c.T);
