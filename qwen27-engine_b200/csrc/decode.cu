@@ -752,10 +752,10 @@ int launch_prefix(DeviceCtx* ctx, const float* qn, const void* kcache, const voi
 int launch_prefix_paged(DeviceCtx* ctx, const float* qn, const void* kpool, const void* vpool, const int* page_table,
                         const int* seq_len, int B, int T, float kq_scale, int nkvh, int n_pages, int max_pages, int max_seq_len,
                         const char* who, PrefixPartials* out, cudaStream_t s) {
-  // A chunk a CTA: one for every SM while that is at most 1,024 positions (a sequence of 1,024: 9.4 us in chunks of 128 and 26.2
-  // in one of 1,024; eight of up to 1,024: 16.5 and 30.8), longer ones when there would be more than sixteen for an SM (16 of up
-  // to 16,384: 87 in chunks of 1,024, 96 of 1,792, 83 of 2,048, 134 of 4,096; 64 of up to 4,096: 131, 141, 137, 159). Four
-  // drafts each; only the longest possible lengths are known here.
+  // A chunk a CTA: one for every SM while that is at most 1,024 positions (a sequence of 1,024: 8.7 us in chunks of 128 and 25.4
+  // in one of 1,024; eight of up to 1,024: 13.0 in chunks of 256, 26.1), longer ones when there would be more than sixteen for an
+  // SM (16 of up to 16,384: 78 in chunks of 1,024, 72 of 2,048, 100 of 1,536, 123 of 4,096; 64 of up to 16,384: 308 in chunks of
+  // 1,792, 345 of 1,024, 330 of 2,048). Four drafts each; only the longest possible lengths are known here.
   const int64_t per_sm = ((int64_t)B * nkvh * max_seq_len + ctx->n_sm - 1) / ctx->n_sm;
   int chunk = (int)std::max<int64_t>(std::min<int64_t>(1024, per_sm), std::min<int64_t>(4096, per_sm / 16));
   chunk = std::max(128, (chunk + 63) / 64 * 64);

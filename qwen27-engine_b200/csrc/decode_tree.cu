@@ -14,12 +14,19 @@
 // may see (past the sequence, on a page that does not exist) are cleared on the way to the tensor core, and drafted V
 // chunks of 16 dims that are not finite are cleared and remembered: the rows that see such a draft get NaN in these dims.
 //
-// Warps 0-7 softmax (two threads a row, 32 columns of a tile each), warp 8 issues the Q K^T MMAs, warp 9 the P V MMAs. f16
-// cache: warp 10 brings the tiles by TMA as the tensor core reads them. q8_0 cache: warps 10-13 turn K and 14-17 V into f16
+// Warps 0-3 softmax of the even tiles and 4-7 of the odd ones, a thread a row; warp 8 issues the Q K^T MMAs, warp 9 the P V MMAs.
+// f16 cache: warp 10 brings the tiles by TMA as the tensor core reads them. q8_0 cache: warps 10-13 turn K and 14-17 V into f16
 // operands, from registers that they load straight from the cache, a tile ahead: through shared
 // memory, which 64 KB of operands a tile written and read again keep busy already, the int8 tile would cost another 68 KB.
-// TMEM: columns 0-255 O (f32), 256-383 two S buffers of 64 columns (f32), 384-511 the Q tile. (P over the scores it was made of
-// saves a store and a load of shared memory, but the next Q K^T then waits for P V: 102 us behind 150,000.)
+// TMEM: columns 0-255 O (f32), 256-383 two buffers of 64 columns for S (f32) and over it P (f16), 384-511 the Q tile.
+//
+// Measured (events, 16 drafts behind 150,000 positions of four heads, 327 MB and 59 GFLOP): 95 us with the GPU cool, 114 in a long
+// run, in which it draws 970 W and lowers its clock to 1.54 GHz: 2.9 TB/s, 0.52 PFLOP/s. At full clock a tile takes 2,600 cycles of an SM;
+// the MMAs are 1,000 of them, MMAs and softmax without the int8 tiles 1,780 (65 us). The following left it at 93 to 98 us and
+// are not in: the next tiles brought into L2 ahead, int8 tiles through TMA into shared memory two ahead, all loads of a tile in a burst,
+// 32-byte loads, no exponentials, 16 converter warps (101). P in shared memory instead of over S: 98 cool and 117 long, a batch of 16
+// sequences 128 long instead of 122. Both warpgroups on every tile, 32 columns a thread: the same at 150,000, 18.2 instead of
+// 19.3 us for 12 drafts behind 20,000 of one f16 head, where a CTA has three tiles.
 #include "cache_ref.h"
 #include "decode_rows.h"
 #include "f16_tile.cuh"
@@ -31,17 +38,16 @@ namespace {
 
 constexpr int QT = TREE_ROWS;    // query rows per CTA
 constexpr float TAU = 5.0f;
-constexpr int NWG = 2, CW = PT / NWG, OW = AD / NWG;  // softmax threads per row; their columns of a tile and of O
+constexpr int NWG = 2, OW = AD / NWG;  // softmax threads per row: of the even and of the odd tiles; their columns of Q and O
 constexpr int NSW = 4 * NWG, MMA_WARP = NSW, PV_WARP = NSW + 1, TMA_WARP = NSW + 2, KCONV_WARP0 = NSW + 2, VCONV_WARP0 = NSW + 6;
-constexpr int N_CONV_WARPS = 4, NK = 3, NV = 2, NP = 2;  // f16 K and V buffers, buffers of P
-enum { B_QFULL = 0, B_KFULL = 1, B_KEMPTY = 4, B_VFULL = 7, B_VEMPTY = 10, B_SFULL = 13, B_SEMPTY = 15, B_PFULL = 17, B_PVDONE = 19, B_ODONE = 21, NBAR = 22 };
+constexpr int N_CONV_WARPS = 4, NK = 3, NV = 3;  // f16 K and V buffers
+enum { B_QFULL = 0, B_KFULL = 1, B_KEMPTY = 4, B_VFULL = 7, B_VEMPTY = 10, B_SFULL = 13, B_PFULL = 15, B_PVDONE = 17, B_ODONE = 19, NBAR = 20 };
 // Shared memory
 constexpr int OFF_K = 0;
 constexpr int OFF_V = OFF_K + NK * KV_BYTES;
-constexpr int P_BYTES = QT * 128;                         // f16 P: [128][64 positions]; first the Q tile on its way to tensor memory
-constexpr int OFF_P = OFF_V + NV * KV_BYTES;
-constexpr int OFF_XCH = OFF_P + NP * P_BYTES;                  // [tile parity][NWG][128] f32
-constexpr int OFF_BAR = OFF_XCH + 2 * NWG * QT * 4;
+constexpr int OFF_STAGE = OFF_V + NV * KV_BYTES;          // the Q tile on its way to tensor memory, 2 KB a softmax warp
+constexpr int OFF_XCH = OFF_STAGE + NSW * 2048;           // f32: [128] reference maxima, [NWG][128] sums
+constexpr int OFF_BAR = OFF_XCH + (1 + NWG) * QT * 4;
 constexpr int OFF_BAD = OFF_BAR + NBAR * 8;               // [16 chunks of 16 dims][2 words]: drafts whose V chunk is not finite
 constexpr int OFF_SKIP = OFF_BAD + 16 * 8;                // [TREE_MAX_TILES / 32] words: tiles on pages that do not exist
 constexpr int OFF_SCAN = OFF_SKIP + TREE_MAX_TILES / 8;   // [32] 64-bit sums
@@ -61,8 +67,10 @@ __device__ __forceinline__ bool elect_one() {
   asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
   return one != 0;
 }
-// the threads of a query row sit in warp q of every softmax warpgroup
-__device__ __forceinline__ void row_sync(int q) { asm volatile("bar.sync %0, %1;" ::"r"(1 + q), "n"(32 * NWG) : "memory"); }
+// The two threads of a query row sit in warp q of either softmax warpgroup. Between them: the reference maximum after a tile is there.
+__device__ __forceinline__ void ref_ready(int q, int parity) { asm volatile("bar.arrive %0, %1;" ::"r"(1 + 2 * q + parity), "n"(64) : "memory"); }
+__device__ __forceinline__ void ref_wait(int q, int parity) { asm volatile("bar.sync %0, %1;" ::"r"(1 + 2 * q + parity), "n"(64) : "memory"); }
+__device__ __forceinline__ void row_sync(int q) { asm volatile("bar.sync %0, %1;" ::"r"(9 + q), "n"(64) : "memory"); }
 __device__ __forceinline__ bool not_finite(uint32_t h2) { return (h2 & 0x7C00u) == 0x7C00u || (h2 & 0x7C000000u) == 0x7C000000u; }
 
 // Clears the 16-byte chunks of a swizzled f16 V tile that may not reach the tensor core: position p (row r of the tile),
@@ -186,20 +194,17 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   const int64_t slot0 = (int64_t)blockIdx.x * QT;  // its rows among the partials
   // Softmax warps q, q + 4 have rows 32 q ..; those past the last row have nothing to do (what the tensor core makes of their rows
   // of Q and P reaches no other row).
-  const int n_active = NWG * min(4, (T * GQA - row0 + 31) / 32);
+  const int n_active = min(4, (T * GQA - row0 + 31) / 32);  // of either warpgroup
   if (tid == 0) {
-    mbar_init(&bar[B_QFULL], n_active);
+    mbar_init(&bar[B_QFULL], NWG * n_active);
     for (int s = 0; s < 3; s++) {
       mbar_init(&bar[B_KFULL + s], Q8 ? N_CONV_WARPS : 1);  // q8_0: the converter warps fill the buffers
       mbar_init(&bar[B_KEMPTY + s], 1);
       mbar_init(&bar[B_VFULL + s], Q8 ? N_CONV_WARPS : 1);
       mbar_init(&bar[B_VEMPTY + s], 1);
     }
-    for (int s = 0; s < 2; s++) {
+    for (int s = 0; s < 2; s++) {  // the buffers of S and P
       mbar_init(&bar[B_SFULL + s], 1);
-      mbar_init(&bar[B_SEMPTY + s], n_active);
-    }
-    for (int s = 0; s < NP; s++) {
       mbar_init(&bar[B_PFULL + s], n_active);
       mbar_init(&bar[B_PVDONE + s], 1);
     }
@@ -216,7 +221,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   __syncthreads();
   auto skipped = [&](int j) { return PAGED && ((((volatile uint32_t*)skip)[j >> 5] >> (j & 31)) & 1); };
 
-  if (warp < NSW && (warp & 3) >= n_active / NWG) {
+  if (warp < NSW && (warp & 3) >= n_active) {
     // no rows
   } else if (warp < NSW) {
     // ================================================================ softmax warps
@@ -232,8 +237,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       // rows, scaled and rounded; rows past 6 T are zero. 32 dims at a time, loaded with eight lanes to 128 contiguous bytes of
       // a row and turned to a row per thread in shared memory (64 bytes a row, 16-byte chunk c of row r at c ^ (r / 2 % 4)).
       constexpr int LD = 2;  // turns whose loads are requested together
-      uint8_t* stage = sgen + OFF_P + warp * 2048;
-      static_assert(NSW * 2048 <= P_BYTES, "staging of the Q tile");
+      uint8_t* stage = sgen + OFF_STAGE + warp * 2048;
 #pragma unroll 1
       for (int c = 0; c < OW / 32; c += LD) {
         float4 x[LD][8];
@@ -273,109 +277,116 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     uint64_t mine = t < T ? p.mask[(size_t)b * T + t] : 0;
     if (T < 64) mine &= ((uint64_t)1 << T) - 1;
 
-    const int col0 = wg * CW;          // this thread's positions of a tile
-    float m_run = M_INIT, m_ref = M_INIT;
+    // The warpgroups take turns at the tiles, so that one's wait for S, its maxima and its exponentials lie under the other's. O
+    // belongs to both: the reference maximum of a row goes from tile to tile, each tile's thread leaves it to the next.
+    float m_ref = M_INIT;  // what l2 is relative to
     uint64_t l2 = pack2(0.f, 0.f);
     const uint64_t log2e2 = pack2(LOG2E, LOG2E);
-
-#pragma unroll 1
-    for (int j = 0; j < nt; j++) {
-      const int slot = j & 1;
-      const int p_tile = (it0 + j) * PT;
-      mbar_wait(&bar[B_SFULL + slot], (j >> 1) & 1, abort_flag, p.c.status);
-      tc_fence_after();
-      float s[CW];
-      {
-        uint32_t v[CW];
-        tmem_ld(tlane + TM_S + slot * PT + col0, v);
-        tc_wait_ld();
-#pragma unroll
-        for (int i = 0; i < CW; i++) s[i] = __uint_as_float(v[i]);
+    auto refer_to = [&](float m) {
+      if (__any_sync(0xffffffffu, m != m_ref)) {
+        const float f = ex2((m_ref - m) * LOG2E);  // 0 on the first move (m_ref = -1e30)
+        l2 = mul2(l2, pack2(f, f));
+        m_ref = m;
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[B_SEMPTY + slot]);  // the buffer is in registers: it can be overwritten
+    };
+#pragma unroll 1
+    for (int j = wg; j < nt; j += NWG) {
+      const int ph = (j >> 1) & 1;
+      const int p_tile = (it0 + j) * PT;
+      mbar_wait(&bar[B_SFULL + wg], ph, abort_flag, p.c.status);
+      tc_fence_after();
       // Columns of the tile that this row sees; only tiles that reach past the prefix (or lie on no page) have others.
-      if (p_tile + PT > zone || skipped(j)) {
+      const bool partly = p_tile + PT > zone || skipped(j);
+      uint64_t vis = ~(uint64_t)0;
+      if (partly) {
         const int j0 = p_tile - first;  // the draft in column 0
-        uint64_t vis = j0 <= -PT ? ~(uint64_t)0 : j0 < 0 ? (mine << -j0) | (((uint64_t)1 << -j0) - 1) : j0 < 64 ? mine >> j0 : 0;
+        vis = j0 <= -PT ? ~(uint64_t)0 : j0 < 0 ? (mine << -j0) | (((uint64_t)1 << -j0) - 1) : j0 < 64 ? mine >> j0 : 0;
         if (n_end - p_tile < PT) vis &= ((uint64_t)1 << (n_end - p_tile)) - 1;
         if (skipped(j)) vis = 0;
-        const uint32_t seen = (uint32_t)(vis >> col0);
-#pragma unroll
-        for (int i = 0; i < CW; i++)
-          if (!((seen >> i) & 1)) s[i] = -INFINITY;
       }
-      float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t v[32];
+      float mt = -INFINITY;
+      auto load_s = [&](int half) {
+        tmem_ld32(tlane + TM_S + wg * PT + 32 * half, v);
+        tc_wait_ld();
+        if (partly) {
+          const uint32_t seen = (uint32_t)(vis >> (32 * half));
 #pragma unroll
-      for (int i = 0; i < CW; i += 4) {
-        mq[0] = fmaxf(mq[0], s[i]);
-        mq[1] = fmaxf(mq[1], s[i + 1]);
-        mq[2] = fmaxf(mq[2], s[i + 2]);
-        mq[3] = fmaxf(mq[3], s[i + 3]);
+          for (int i = 0; i < 32; i++)
+            if (!((seen >> i) & 1)) v[i] = 0xFF800000u;
+        }
+      };
+#pragma unroll
+      for (int half = 1; half >= 0; half--) {
+        load_s(half);
+        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 32; i++) mq[i & 3] = fmaxf(mq[i & 3], __uint_as_float(v[i]));
+        mt = fmaxf(mt, fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])));
       }
-      float mt = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
-      // row maximum over the threads of the row; the buffer alternates with the tile
-      xch[(slot * NWG + wg) * QT + r] = mt;
-      row_sync(q);
-#pragma unroll
-      for (int o = 1; o < NWG; o++) mt = fmaxf(mt, xch[(slot * NWG + ((wg + o) % NWG)) * QT + r]);
-      m_run = fmaxf(m_run, mt);
 
-      // Move the reference max when the true max has run away from it (and on the first tile with a visible column). The
-      // threads of a row hold the same m_run and m_ref, so their warps take the same branch.
-      const bool want = m_run > m_ref + TAU;
-      if (__any_sync(0xffffffffu, want)) {
-        const float f = ex2((m_ref - m_run) * LOG2E);  // 0 on the first move (m_ref = -1e30)
-        m_ref = m_run;
-        l2 = mul2(l2, pack2(f, f));
+      // The reference of a row moves when the maximum has run away from it (and on the first tile with a visible column).
+      if (j > 0) ref_wait(q, wg ^ 1);
+      float m = j > 0 ? xch[r] : M_INIT;
+      if (__any_sync(0xffffffffu, mt > m + TAU)) {
+        const float f = ex2((m - fmaxf(m, mt)) * LOG2E);
+        m = fmaxf(m, mt);
         if (j > 0) {
           // O holds the sum of tiles < j once the P V of tile j-1 has completed
-          mbar_wait(&bar[B_PVDONE + (slot ^ 1)], ((j - 1) >> 1) & 1, abort_flag, p.c.status);
+          mbar_wait(&bar[B_PVDONE + (wg ^ 1)], ((j - 1) >> 1) & 1, abort_flag, p.c.status);
           tc_fence_after();
-          rescale_o_f16(tlane + TM_O + wg * OW, f, OW / 32);
+          rescale_o_f16(tlane + TM_O, f, AD / 32);
           tc_wait_st();
           tc_fence_before();
         }
       }
+      xch[r] = m;
+      if (j + 1 < nt) ref_ready(q, wg);
+      refer_to(m);
 
-      // P = exp(s - m_ref): f32 row sum, f16 for the P V MMA (16-byte chunks CW/8 wg .. of the row)
-      mbar_wait(&bar[B_PVDONE + slot], ((j >> 1) & 1) ^ 1, abort_flag, p.c.status);  // P V of tile j-2 has read the buffer
-      const float nmb = -m_ref * LOG2E;
+      // P = exp(s - m): f32 row sum, f16 for the P V MMA
+      const float nmb = -m * LOG2E;
       const uint64_t nmb2 = pack2(nmb, nmb);
 #pragma unroll
-      for (int c = 0; c < CW / 8; c++) {
-        uint32_t w[4];
+      for (int half = 0; half < 2; half++) {
+        if (half) load_s(half);
+        uint32_t w[16];
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          float a0, a1;
-          unpack2(fma2(pack2(s[c * 8 + 2 * k], s[c * 8 + 2 * k + 1]), log2e2, nmb2), a0, a1);
-          const float e0 = ex2(a0), e1 = ex2(a1);
-          l2 = add2(l2, pack2(e0, e1));
-          w[k] = pack_h2(e0, e1);
+        for (int c = 0; c < 4; c++) {
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            float a0, a1;
+            unpack2(fma2(pack2(__uint_as_float(v[c * 8 + 2 * k]), __uint_as_float(v[c * 8 + 2 * k + 1])), log2e2, nmb2), a0, a1);
+            const float e0 = ex2(a0), e1 = ex2(a1);
+            l2 = add2(l2, pack2(e0, e1));
+            w[4 * c + k] = pack_h2(e0, e1);
+          }
         }
-        *(uint4*)(sgen + OFF_P + slot * P_BYTES + swz128(r, CW / 8 * wg + c)) = make_uint4(w[0], w[1], w[2], w[3]);
+        tmem_st16(tlane + TM_S + wg * PT + 16 * half, w);  // over the scores that it was made of
       }
       if (!Q8 && p_tile + PT > zone) {  // f16 cache: V lies in the operand buffer as it came (the converters do this for q8_0)
         const int vb = j % NV;
         mbar_wait(&bar[B_VFULL + vb], (j / NV) & 1, abort_flag, p.c.status);
-        for (int u = (wg * (n_active / NWG) + q) * 32 + lane; u < 4 * PT; u += 32 * n_active)  // (segment, row)
+        for (int u = q * 32 + lane; u < 4 * PT; u += 32 * n_active)  // (segment, row)
           clean_v_row(sgen + OFF_V + vb * KV_BYTES + (u >> 6) * SEGK + (u & 63) * 128, u & 63, u >> 6, zone - p_tile, n_end - p_tile,
                       p_tile + (u & 63) - first, bad);
       }
-      fence_proxy_async();
+      if (!Q8) fence_proxy_async();
+      tc_wait_st();
+      tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar[B_PFULL + slot]);
+      if (lane == 0) mbar_arrive(&bar[B_PFULL + wg]);
     }
 
-    // ---- epilogue: the unnormalised partial of this share
+    // ---- epilogue: the unnormalised partial of this part
+    row_sync(q);
+    refer_to(xch[r]);  // as the last tile left it
     float la, lb;
     unpack2(l2, la, lb);
     float l = la + lb;
-    xch[((nt & 1) * NWG + wg) * QT + r] = l;
+    xch[(1 + wg) * QT + r] = l;
     row_sync(q);
-#pragma unroll
-    for (int o = 1; o < NWG; o++) l += xch[((nt & 1) * NWG + ((wg + o) % NWG)) * QT + r];
+    l += xch[(1 + (wg ^ 1)) * QT + r];
     if (wg == 0 && t < T) p.part_ml[slot0 + r] = make_float2(m_ref, l);
     mbar_wait(&bar[B_ODONE], 0, abort_flag, p.c.status);
     tc_fence_after();
@@ -419,7 +430,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     for (int j = 0; j < nt; j++) {
       const int ss = j & 1, sph = (j >> 1) & 1;                         // S buffer
       mbar_wait(&bar[B_KFULL + st], ph, abort_flag, p.c.status);
-      mbar_wait(&bar[B_SEMPTY + ss], sph ^ 1, abort_flag, p.c.status);
+      mbar_wait(&bar[B_PVDONE + ss], sph ^ 1, abort_flag, p.c.status);  // P V of tile j-2 has read P there
       tc_fence_after();
       if (issuer) {
 #pragma unroll
@@ -435,7 +446,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
   } else if (warp == PV_WARP) {
     // ================================================================ P V issuer
     const bool issuer = elect_one();
-    const uint64_t desc_p = umma_desc_sw128(sbase + OFF_P, 16, 1024), desc_v = umma_desc_sw128(sbase + OFF_V, SEGK, 1024);
+    const uint64_t desc_v = umma_desc_sw128(sbase + OFF_V, SEGK, 1024);
     int st = 0, ph = 0;  // V buffer and its phase
 #pragma unroll 1
     for (int j = 0; j < nt; j++) {
@@ -446,7 +457,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       if (issuer) {
 #pragma unroll
         for (int kk = 0; kk < PT / 16; kk++)
-          tc_mma_f16(tmem + TM_O, desc_p + (uint64_t)(pb * (P_BYTES / 16) + kk * 2), desc_v + (uint64_t)(st * (KV_BYTES / 16) + kk * 128),
+          tc_mma_f16_ts(tmem + TM_O, tmem + TM_S + pb * PT + kk * 8, desc_v + (uint64_t)(st * (KV_BYTES / 16) + kk * 128),
                      IDESC_PV, (j > 0 || kk > 0) ? 1u : 0u);
         tc_commit(&bar[B_PVDONE + pb]);
         tc_commit(&bar[B_VEMPTY + st]);
