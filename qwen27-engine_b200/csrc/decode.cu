@@ -758,7 +758,8 @@ int launch_prefix_paged(DeviceCtx* ctx, const float* qn, const void* kpool, cons
   // 1,792, 345 of 1,024, 330 of 2,048). Four drafts each; only the longest possible lengths are known here.
   const int64_t per_sm = ((int64_t)B * nkvh * max_seq_len + ctx->n_sm - 1) / ctx->n_sm;
   int chunk = (int)std::max<int64_t>(std::min<int64_t>(1024, per_sm), std::min<int64_t>(4096, per_sm / 16));
-  chunk = std::max(128, (chunk + 63) / 64 * 64);
+  chunk = std::max(128, (int)std::min<int64_t>(max_seq_len, std::max<int64_t>(chunk, per_sm / 64)));  // (at most 64 an SM: 240 MB of partials)
+  chunk = (chunk + 63) / 64 * 64;
   const int nch = (max_seq_len + chunk - 1) / chunk;
   float* part;
   if (int rc = paged_ws(ctx, (size_t)B * nkvh * nch * MAXR * PROW, &part, who)) return rc;

@@ -483,3 +483,105 @@ def test_few_drafts_poisoned_rows_and_runaway_scores(q27, paged, q8):
     tol = ref[1] * (torch.expm1(2 * ds) + 2.0 ** -10)[..., None] + (ref[3] * 2.0 ** -25)[..., None] + ref[0].abs() * 2.0 ** -11 + 2.0 ** -25
     assert ((o.view(ref[0].shape).double() - ref[0]).abs() <= tol).all()
     assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("paged,q8", [(False, True), (False, False), (True, True)])
+def test_few_drafts_that_see_what_is_not_finite(q27, paged, q8):
+    T, n = 4, 390
+    st = H.Store([n], T, 2, paged, q8, seed=3)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    mask = H.mask_tensor([[0b0001, 0b0010, 0b0111, 0b1000]])
+    qn, qg = H.queries(st, 3)
+    clean = H.call_tree(q27, st, kc, vc, qn, qg, mask)[0]
+    for which in ("k", "v"):
+        k2, v2 = kc.clone(), vc.clone()
+        for h in range(2):
+            st.poison(k2 if which == "k" else v2, 0, h, [n - T])
+        o = H.call_tree(q27, st, k2, v2, qn, qg, mask)[0]
+        for t in range(T):
+            assert torch.isnan(o[t]).all() if t in (0, 2) else torch.equal(o[t], clean[t]), (which, t)
+
+
+def test_few_drafts_no_length_and_bad_pages(q27):
+    """Sequences shorter than their drafts, of no length, of a negative one; page indices outside the pool are reported, and the other
+    sequences keep their results."""
+    T = 4
+    st = H.Store([0, 3, 300, 4, 700], T, 2, True, True, seed=2)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    masks = [[0b1111, 0b0011, 0b1100, 0b1000]] * 5
+    qn, qg = H.queries(st, 3)
+    mask = H.mask_tensor(masks)
+    o = H.call_tree(q27, st, kc, vc, qn, qg, mask)
+    assert (o[0] == 0).all()
+    H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+    st.seq_len[0] = -7
+    assert torch.equal(H.call_tree(q27, st, kc, vc, qn, qg, mask), o)
+    assert q27.device_status() == 0
+    for seq, page in ((4, 0), (4, 2), (2, 1)):  # in the prefix, and under the drafts (positions 696 .. and 296 ..)
+        good = st.table[seq, page].item()
+        for bad in (-5, st.n_pages, 2 ** 31 - 1):
+            st.table[seq, page] = bad
+            got = H.call_tree(q27, st, kc, vc, qn, qg, mask)
+            assert q27.device_status() == 2
+            assert all(torch.equal(got[b], o[b]) for b in range(5) if b != seq)
+        st.table[seq, page] = good
+    assert torch.equal(H.call_tree(q27, st, kc, vc, qn, qg, mask), o)
+
+
+@pytest.mark.parametrize("q8", [True, False])
+def test_few_drafts_replayed_on_another_stream(q27, q8):
+    """A captured call sees new positions and masks, with the query still being written before it; f16 and q8_1 output."""
+    T, nkvh = 3, 4
+    st = H.Store([1500], T, nkvh, False, q8, seed=4)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    qn, qg = H.queries(st, 3)
+    mask = H.mask_tensor(H.random_masks(1, T, seed=1))
+    o = torch.zeros((1, T, st.nqh, H.AD), dtype=torch.float16, device="cuda")
+    xq, xd = torch.zeros(o.shape, dtype=torch.int8, device="cuda"), torch.zeros(o.numel() // 32, device="cuda")
+    qn2 = torch.zeros_like(qn)
+
+    def step():
+        qn2.zero_()
+        for _ in range(10):
+            qn2.add_(qn, alpha=0.05)
+        qn2.copy_(qn)
+        H.call_tree(q27, st, kc, vc, qn2, qg, mask, o)
+        H.call_tree(q27, st, kc, vc, qn2, qg, mask, None, xq, xd)
+
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for n, seed in ((1500, 1), (T, 2), (64, 3), (T + 1, 4), (777, 5)):
+        masks = H.random_masks(1, T, seed=seed)
+        st.lens = [n]
+        st.pos0.fill_(n - T)
+        mask.copy_(H.mask_tensor(masks))
+        graph.replay()
+        H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+        d, ob = xd.view(-1, 1).double(), o.view(-1, 32).double()
+        assert ((xq.view(-1, 32).double() * d - ob).abs() <= d * 0.501 + ob.abs() * 2.0 ** -10 + 1e-7).all()
+
+
+@pytest.mark.parametrize("mode", ["0", "1"])
+def test_few_drafts_in_other_launch_modes(q27, mode):
+    import os
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+    subset = ["tests/test_gpu_tree.py::test_few_drafts_of_a_batch", "tests/test_gpu_tree.py::test_few_drafts_replayed_on_another_stream"]
+    r = subprocess.run([sys.executable, "-m", "pytest", "-x", "-q", "-m", "gpu", "-p", "no:cacheprovider"] + subset, cwd=ROOT,
+                       env=dict(os.environ, Q27_PDL=mode), capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout[-3000:] + r.stderr[-1000:]
+    assert " passed" in r.stdout
