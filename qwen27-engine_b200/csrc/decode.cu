@@ -136,12 +136,13 @@ __device__ __forceinline__ int ks_dim0(int ks, int tg) {
 }
 
 // NT = 8-row groups of query rows (ceil(6 T / 8)). PAGED: batched decode over 256-position pages
-// (q8_0 only). Q8: q8_0 cache (else f16). SEL: every token (grid z) attends its own list of blocks, a chunk is a part of it.
-template <int NT, bool PAGED, bool Q8, bool SEL = false>
+// (q8_0 only). Q8: q8_0 cache (else f16). LIST: every token (grid z) attends its own list of blocks, a chunk is a part of it.
+template <int NT, bool PAGED, bool Q8, Rows ROWS = Rows::ALL>
 __global__ void __launch_bounds__(N_THREADS, 1)
 decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_ks,
               const __grid_constant__ CUtensorMap tm_vv, const __grid_constant__ CUtensorMap tm_vs,
-              const DecodeParams p) {
+              const typename ParamsOf<ROWS>::type p) {
+  constexpr bool SEL = ROWS == Rows::LIST;
   using G = Geo<Q8>;
   constexpr int NSTAGE = G::NSTAGE, NFULL = G::NFULL;
   extern __shared__ uint8_t smem_raw[];
@@ -168,12 +169,14 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
   const int ch = blockIdx.x, kh = blockIdx.y;
   const int T = p.T, R = GQA * T;
   const int seq = PAGED || SEL ? blockIdx.z : 0;
-  const int pos0 = SEL ? sel_pos(p, PAGED, seq) : PAGED ? p.seq_len[seq] - T : *p.pos0;
+  int pos0;
+  if constexpr (SEL) pos0 = sel_pos(p, PAGED, seq);
+  else pos0 = PAGED ? p.seq_len[seq] - T : *p.pos0;
   const float* qn = p.qn + (size_t)seq * T * p.nqh * AD;
   const int g = lane >> 2, tg = lane & 3;
 
   // Local rows to attend, and this CTA's chunk [c0, c1) of them (multiples of TILE).
-  int n = pos0 + T - p.hold - p.base_pos;
+  int n = pos0 + (ROWS == Rows::PREFIX ? 0 : T) - p.base_pos;
   if (p.n_local >= 0) n = min(n, p.n_local);
   n = max(0, min(n, p.n_ctx));
   int chunk;
@@ -194,10 +197,12 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
     return;
   }
   int ntiles = (c1 - c0 + TILE - 1) / TILE;
-  int* const list = (int*)(sgen + OFF_LIST);
-  if (SEL && warp == 0) {
-    const int c = collect_blocks(p, PAGED, seq, kh, ch * p.chunk_len, min(p.sel_k, (ch + 1) * p.chunk_len), n, list);
-    if (lane == 0) list[SEL_CHUNK] = c;
+  int* const list = (int*)(sgen + OFF_LIST);  // (LIST)
+  if constexpr (SEL) {
+    if (warp == 0) {
+      const int c = collect_blocks(p, PAGED, seq, kh, ch * p.chunk_len, min(p.sel_k, (ch + 1) * p.chunk_len), n, list);
+      if (lane == 0) list[SEL_CHUNK] = c;
+    }
   }
 
   __syncthreads();
@@ -556,8 +561,9 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
         f[0] = ex2((m[nt][e] - M) * LOG2E);
 #pragma unroll
         for (int k = 1; k < NGROUP; k++) f[k] = ex2((mg[k] - M) * LOG2E);
-        const size_t at = ((size_t)seq * p.nqh + kh * GQA + r) * p.nch + ch;  // SEL: [row][chunk]
-        float* po = SEL ? p.part_o + at * AD - 2 : out + (size_t)r * PROW;
+        const size_t at = ((size_t)seq * p.nqh + kh * GQA + r) * p.nch + ch;  // LIST: [row][chunk]
+        float* po = out + (size_t)r * PROW;
+        if constexpr (SEL) po = p.part_o + at * AD - 2;
 #pragma unroll
         for (int mt = 0; mt < 4; mt++) {
           const int d = 64 * wq + 8 * g + 2 * mt;
@@ -578,7 +584,7 @@ decode_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__
             for (int w = 0; w < 4; w++) lk += ldsf(sbase + OFF_L + ((k * 4 + w) * MAXR + r) * 4);
             lsum += lk * f[k];
           }
-          if (SEL) {
+          if constexpr (SEL) {
             p.part_ml[at] = make_float2(M, lsum);
           } else {
             po[0] = M;
@@ -601,7 +607,7 @@ int get_tmaps(const void* cache, int nkvh, int n_ctx, bool q8, CUtensorMap* vals
 // Per-device one-time set-up flags of this file's kernels (attribute opt-ins), safe from several threads.
 std::mutex g_setup_mu;
 
-template <int NT, bool PAGED, bool Q8>
+template <int NT, bool PAGED, bool Q8, Rows ROWS>
 int launch_decode(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                   const DecodeParams& p, int nseq, cudaStream_t s) {
   static bool attr[64] = {};
@@ -610,21 +616,21 @@ int launch_decode(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMa
   {
     std::lock_guard<std::mutex> lock(g_setup_mu);
     if (!attr[dev]) {
-      Q27B_CK(cudaFuncSetAttribute(decode_kernel<NT, PAGED, Q8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+      Q27B_CK(cudaFuncSetAttribute(decode_kernel<NT, PAGED, Q8, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
       attr[dev] = true;
     }
   }
-  Q27B_CK(launch_step(decode_kernel<NT, PAGED, Q8>, dim3(p.nch, p.nkvh, nseq), dim3(N_THREADS), SMEM_BYTES, s, *kv, *ks, *vv,
+  Q27B_CK(launch_step(decode_kernel<NT, PAGED, Q8, ROWS>, dim3(p.nch, p.nkvh, nseq), dim3(N_THREADS), SMEM_BYTES, s, *kv, *ks, *vv,
                      *vs, p));
   return Q27B_OK;
 }
-template <bool PAGED, bool Q8>
+template <bool PAGED, bool Q8, Rows ROWS = Rows::ALL>
 int launch_decode_t(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                     const DecodeParams& p, int nseq, cudaStream_t s) {
   const int nt = (GQA * p.T + 7) / 8;
-  if (nt == 1) return launch_decode<1, PAGED, Q8>(kv, ks, vv, vs, p, nseq, s);
-  if (nt == 2) return launch_decode<2, PAGED, Q8>(kv, ks, vv, vs, p, nseq, s);
-  return launch_decode<3, PAGED, Q8>(kv, ks, vv, vs, p, nseq, s);
+  if (nt == 1) return launch_decode<1, PAGED, Q8, ROWS>(kv, ks, vv, vs, p, nseq, s);
+  if (nt == 2) return launch_decode<2, PAGED, Q8, ROWS>(kv, ks, vv, vs, p, nseq, s);
+  return launch_decode<3, PAGED, Q8, ROWS>(kv, ks, vv, vs, p, nseq, s);
 }
 
 // Which split-K kernel serves a q8_0 cache: the warp-specialised kernel of decode_ws.cu unless
@@ -743,10 +749,10 @@ int launch_prefix(DeviceCtx* ctx, const float* qn, const void* kcache, const voi
   if (int rc = get_tmaps(vcache, nkvh, n_ctx, q8, &vv, &vs)) return rc;
   DecodeParams p = {};
   p.qn = qn; p.part = part; p.pos0 = pos0; p.status = ctx->status; p.T = T; p.nqh = nkvh * GQA; p.nkvh = nkvh; p.n_ctx = n_ctx;
-  p.nch = ctx->n_sm / nkvh; p.kq_scale = kq_scale; p.n_local = -1; p.hold = T;
+  p.nch = ctx->n_sm / nkvh; p.kq_scale = kq_scale; p.n_local = -1;
   *out = {part, p.nch, 0};
   // (equal static shares: the same bits on every run)
-  return q8 ? launch_decode_ws(&kv, &ks, &vv, &vs, p, false, 1, s) : launch_decode_t<false, false>(&kv, &ks, &vv, &vs, p, 1, s);
+  return q8 ? launch_prefix_ws(&kv, &ks, &vv, &vs, p, 1, s) : launch_decode_t<false, false, Rows::PREFIX>(&kv, &ks, &vv, &vs, p, 1, s);
 }
 
 int launch_prefix_paged(DeviceCtx* ctx, const float* qn, const void* kpool, const void* vpool, const int* page_table,
@@ -768,26 +774,26 @@ int launch_prefix_paged(DeviceCtx* ctx, const float* qn, const void* kpool, cons
   if (int rc = get_tmaps(vpool, nkvh, n_pages * Q27B_PAGE, true, &vv, &vs)) return rc;
   DecodeParams p = {};
   p.qn = qn; p.part = part; p.status = ctx->status; p.T = T; p.nqh = nkvh * GQA; p.nkvh = nkvh; p.n_ctx = max_seq_len; p.nch = nch;
-  p.kq_scale = kq_scale; p.n_local = -1; p.hold = T; p.page_table = page_table; p.seq_len = seq_len; p.max_pages = max_pages;
+  p.kq_scale = kq_scale; p.n_local = -1; p.page_table = page_table; p.seq_len = seq_len; p.max_pages = max_pages;
   p.n_pages = n_pages; p.chunk_len = chunk;
   *out = {part, nch, chunk};
   const bool spread = (int64_t)nch * nkvh * B <= ctx->n_sm;
-  return launch_decode_ws(&kv, &ks, &vv, &vs, p, true, B, s, spread ? WsGroups::SPREAD : WsGroups::PAIRED);
+  return launch_prefix_ws_paged(&kv, &ks, &vv, &vs, p, B, s, spread ? WsGroups::SPREAD : WsGroups::PAIRED);
 }
 
-int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const DecodeParams& p, int nseq, cudaStream_t s) {
+int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const ListParams& p, int nseq, cudaStream_t s) {
   static bool attr[64] = {};
   int dev;
   Q27B_CK(cudaGetDevice(&dev));
   {
     std::lock_guard<std::mutex> lock(g_setup_mu);
     if (!attr[dev]) {
-      Q27B_CK(cudaFuncSetAttribute(decode_kernel<1, false, false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_SMEM_BYTES));
+      Q27B_CK(cudaFuncSetAttribute(decode_kernel<1, false, false, Rows::LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, SEL_SMEM_BYTES));
       attr[dev] = true;
     }
   }
   // (the maps of scales are not read)
-  Q27B_CK(launch_step(decode_kernel<1, false, false, true>, dim3(p.nch, p.nkvh, nseq), dim3(N_THREADS), SEL_SMEM_BYTES, s, *kv, *kv, *vv, *vv, p));
+  Q27B_CK(launch_step(decode_kernel<1, false, false, Rows::LIST>, dim3(p.nch, p.nkvh, nseq), dim3(N_THREADS), SEL_SMEM_BYTES, s, *kv, *kv, *vv, *vv, p));
   return Q27B_OK;
 }
 

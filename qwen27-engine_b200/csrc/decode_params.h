@@ -14,7 +14,6 @@ struct DecodeParams {
   float kq_scale;
   int base_pos;      // global position of local cache row 0
   int n_local;       // local rows to attend; < 0: all rows up to *pos0 + T
-  int hold;          // rows at the end that are left out: T for the prefix alone (launch_prefix)
   // paged / batched variant: grid (chunks, nkvh, B), fixed chunk length, rows through the page table
   const int* page_table;  // [B][max_pages]
   const int* seq_len;     // [B], counts the T new tokens
@@ -22,15 +21,25 @@ struct DecodeParams {
   // Tile pool of the warp-specialised kernel (one sequence only): [KV head] tiles drawn so far,
   // [32] CTAs that are done; all zero between launches. Null: every CTA keeps to its own share.
   int* sched;
-  // Lists of blocks (decode over selected blocks, T = 1, one "sequence" per (sequence, token)): [B][sel_T][nkvh][sel_k]
-  // 64-position blocks, -1 = none, chunk_len entries to a chunk; the partials go to part_o [row][nch][256] and part_ml [row][nch].
+  // measurement hook (null in normal use): [CTA][8] globaltimer stamps of the warp-specialised kernel
+  unsigned long long* trace;
+};
+
+// Which rows the tokens of a decode kernel attend: up to their own (attn_decode), those before all of them (launch_prefix), or
+// those of a list of blocks. The other two are kernels of their own, with their parameters apart: with a list's fields in
+// DecodeParams and its code beside theirs, ptxas arranged the kernels of attn_decode otherwise, and they took longer (f16, 32,768
+// positions, one and four tokens: 29.6 and 36.6 us a call without, 33.8 and 40.4 with; q8_0, 150,000, four: 76.8 and 81.6).
+enum class Rows { ALL, PREFIX, LIST };
+// Lists of blocks (T = 1, one "sequence" per (sequence, token)): [B][sel_T][nkvh][sel_k] 64-position blocks, -1 = none, chunk_len
+// entries to a chunk; the partials go to part_o [row][nch][256] and part_ml [row][nch].
+struct ListParams : DecodeParams {
   const int* sel;
   int sel_k, sel_T;
   float* part_o;
   float2* part_ml;
-  // measurement hook (null in normal use): [CTA][8] globaltimer stamps of the warp-specialised kernel
-  unsigned long long* trace;
 };
+template <Rows ROWS> struct ParamsOf { using type = DecodeParams; };
+template <> struct ParamsOf<Rows::LIST> { using type = ListParams; };
 
 // One sequence: its tiles of 64 positions are dealt out to the nch chunks of a KV head in equal shares of up to
 // ceil(tiles / nch) tiles; above this share the chunks keep back a common pool (decode_ws.cu) and every chunk has tiles.
@@ -57,14 +66,19 @@ int launch_decode_tc(const CUtensorMap* kv, const CUtensorMap* ks, const CUtenso
 enum class WsGroups { TWO, PAIRED, SPREAD };
 int launch_decode_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                      const DecodeParams& p, bool paged, int nseq, cudaStream_t s, WsGroups groups = WsGroups::TWO);
+// The same for the rows before the T tokens alone.
+int launch_prefix_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                     const DecodeParams& p, int nseq, cudaStream_t s);
+int launch_prefix_ws_paged(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                           const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups);
 // The same with the P V contraction on tcgen05 (decode_wt.cu).
 int launch_decode_wt(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                      const DecodeParams& p, bool paged, int nseq, cudaStream_t s);
 // Decode over lists of blocks: the warp-specialised kernel (q8_0, p.page_table null: contiguous; groups as above) and the
 // single-role kernel of decode.cu (f16 caches). nseq = B * sel_T.
 int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
-                     const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups);
-int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const DecodeParams& p, int nseq, cudaStream_t s);
+                     const ListParams& p, int nseq, cudaStream_t s, WsGroups groups);
+int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const ListParams& p, int nseq, cudaStream_t s);
 // The attention of T = 1..4 tokens to the rows before them alone, by the kernels of a decode call (q8_0: the warp-specialised one;
 // f16: decode.cu); partials [sequence][KV head][chunk][24][258].
 struct PrefixPartials {

@@ -314,7 +314,7 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   p.nsplit = (p.k + chunk - 1) / chunk;
   p.part_o = part;
   p.part_ml = (float2*)(part + rows * p.nsplit * AD);
-  DecodeParams d = {};
+  ListParams d = {};
   d.qn = p.qn; d.pos0 = c.pos0; d.status = c.status; d.T = 1; d.nqh = c.nkvh * GQA; d.nkvh = c.nkvh; d.n_ctx = c.n_ctx;
   d.nch = p.nsplit; d.kq_scale = p.kq_scale; d.n_local = -1; d.page_table = c.page_table; d.seq_len = c.seq_len;
   d.max_pages = c.max_pages; d.n_pages = c.n_pages; d.chunk_len = chunk; d.sel = p.sel; d.sel_k = p.k; d.sel_T = c.T;

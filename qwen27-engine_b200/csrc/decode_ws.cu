@@ -154,14 +154,15 @@ __device__ __forceinline__ int slot_row(int s) { return (s & 8) | ((s & 1) << 2)
 // (a 16-byte load is 16 dims = 4 k-steps).
 __device__ __forceinline__ int ks_dim0(int ks, int tg) { return 128 * (ks >> 3) + 64 * ((ks >> 2) & 1) + 16 * tg + 4 * (ks & 3); }
 
-// NT = 8-row groups of query rows (ceil(6 T / 8)). PAGED: batched decode over 256-position pages. SEL: every (sequence, token)
+// NT = 8-row groups of query rows (ceil(6 T / 8)). PAGED: batched decode over 256-position pages. LIST: every (sequence, token)
 // attends its own list of blocks; grid z is that pair, a chunk is a part of the list, and the tile numbers in the groups' queues
 // are those of the list.
-template <int NT, bool PAGED, int NG, bool SEL = false>
+template <int NT, bool PAGED, int NG, Rows ROWS = Rows::ALL>
 __global__ void __launch_bounds__(256 * NG, 3 - NG)
 decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_ks,
                  const __grid_constant__ CUtensorMap tm_vv, const __grid_constant__ CUtensorMap tm_vs,
-                 const DecodeParams p) {
+                 const typename ParamsOf<ROWS>::type p) {
+  constexpr bool SEL = ROWS == Rows::LIST;
   using L = Lay<NG>;
   constexpr int WS_THREADS = L::THREADS;
   constexpr int OFF_KRING = L::OFF_KRING, OFF_VRING = L::OFF_VRING, OFF_Q = L::OFF_Q, OFF_P = L::OFF_P, OFF_MAX = L::OFF_MAX,
@@ -212,7 +213,9 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
     qv[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < R) qv[j] = *(const float4*)(qn + ((size_t)(r / GQA) * p.nqh + kh * GQA + r % GQA) * AD + 4 * c4);
   }
-  const int pos0 = SEL ? sel_pos(p, PAGED, seq) : PAGED ? p.seq_len[seq] - T : *p.pos0;
+  int pos0;
+  if constexpr (SEL) pos0 = sel_pos(p, PAGED, seq);
+  else pos0 = PAGED ? p.seq_len[seq] - T : *p.pos0;
 
   // Local rows to attend (n) and the tiles of this CTA. Tiles are numbered over the local rows of the
   // sequence (tile t = rows 64 t ..). A CTA owns the `n_static` tiles from `t_first` on; one sequence
@@ -220,12 +223,12 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   // from one by one when their own tiles are done (the SMs do not stream at equal rates: with equal
   // static shares the slowest CTA of a 150k-position call ends 5 us after the median one). A CTA
   // folds whatever tiles it gets into one partial: the log-sum-exp merge does not care which.
-  int n = pos0 + T - p.hold - p.base_pos;
+  int n = pos0 + (ROWS == Rows::PREFIX ? 0 : T) - p.base_pos;
   if (p.n_local >= 0) n = min(n, p.n_local);
   n = max(0, min(n, p.n_ctx));
   int t_first, n_static, n_end, pool0, ntiles_all;
-  int* const list = (int*)(sgen + L::OFF_LIST);
-  if (SEL) {
+  int* const list = (int*)(sgen + L::OFF_LIST);  // (LIST)
+  if constexpr (SEL) {
     t_first = n_static = ntiles_all = pool0 = 0;
     n_end = n;
     if (warp == 0) {
@@ -267,7 +270,9 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
     int row = kh * p.n_ctx + t * TILE;
     if (PAGED) {  // a tile never straddles a page (64 | 256)
       const int pp = t * TILE;
-      int pg = p.page_table[(size_t)(SEL ? seq / p.sel_T : seq) * p.max_pages + pp / Q27B_PAGE];
+      int owner = seq;
+      if constexpr (SEL) owner = seq / p.sel_T;
+      int pg = p.page_table[(size_t)owner * p.max_pages + pp / Q27B_PAGE];
       if (pg < 0 || pg >= p.n_pages) {  // never read outside the pool: flag it and read page 0
         atomicOr(p.status, ST_BAD_PAGE);
         pg = 0;
@@ -807,7 +812,7 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
     }
   }
   bar_sync(BAR_PVALL, 128 * NG);
-  if (SEL) {  // [row][chunk]: row = (sequence, token, head)
+  if constexpr (SEL) {  // [row][chunk]: row = (sequence, token, head)
     const size_t row0 = (size_t)seq * p.nqh + kh * GQA;
     for (int i = tid - PV0; i < GQA * (PROW / 2); i += 128 * NG) {
       const int r = i / (PROW / 2), c = i % (PROW / 2);
@@ -826,77 +831,98 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
 constexpr int SPREAD_SMEM_BYTES = 116 * 1024;
 static_assert(SPREAD_SMEM_BYTES >= Lay<1>::SMEM_BYTES && 2 * (SPREAD_SMEM_BYTES + 1024) > 228 * 1024, "one CTA per SM");
 
-template <int NT, int NG>
+template <int NT, bool PAGED, int NG, Rows ROWS>
 int launch_ws_nt(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
-                 const DecodeParams& p, bool paged, int nseq, cudaStream_t s, int smem = Lay<NG>::SMEM_BYTES) {
-  const dim3 grid(p.nch, p.nkvh, nseq);
-  if (paged)
-    Q27B_CK(launch_step(decode_ws_kernel<NT, true, NG>, grid, dim3(Lay<NG>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
-  else
-    Q27B_CK(launch_step(decode_ws_kernel<NT, false, NG>, grid, dim3(Lay<NG>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
+                 const DecodeParams& p, int nseq, cudaStream_t s, int smem) {
+  Q27B_CK(launch_step(decode_ws_kernel<NT, PAGED, NG, ROWS>, dim3(p.nch, p.nkvh, nseq), dim3(Lay<NG>::THREADS), smem, s, *kv, *ks,
+                      *vv, *vs, p));
   return Q27B_OK;
 }
+template <bool PAGED, int NG, Rows ROWS>
+int launch_ws_t(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                const DecodeParams& p, int nseq, cudaStream_t s, int smem = Lay<NG>::SMEM_BYTES) {
+  const int nt = (GQA * p.T + 7) / 8;
+  if (nt == 1) return launch_ws_nt<1, PAGED, NG, ROWS>(kv, ks, vv, vs, p, nseq, s, smem);
+  if (nt == 2) return launch_ws_nt<2, PAGED, NG, ROWS>(kv, ks, vv, vs, p, nseq, s, smem);
+  return launch_ws_nt<3, PAGED, NG, ROWS>(kv, ks, vv, vs, p, nseq, s, smem);
+}
+int smem_of(WsGroups groups) { return groups == WsGroups::SPREAD ? SPREAD_SMEM_BYTES : Lay<1>::SMEM_BYTES; }  // one tile group
 
 template <bool PAGED, int NG>
 int blocks_attr() {
-  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, Rows::LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                NG == 1 ? SPREAD_SMEM_BYTES : Lay<NG>::SEL_SMEM_BYTES));
   if (NG == 1)
-    Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, true>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, Rows::LIST>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
   return Q27B_OK;
 }
 
-template <int NT, bool PAGED, int NG>
+template <int NT, bool PAGED, int NG, Rows ROWS>
 int ws_attr() {
-  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<NT, PAGED, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<NT, PAGED, NG, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                NG == 1 ? SPREAD_SMEM_BYTES : Lay<NG>::SMEM_BYTES));
   if (NG == 1)  // two CTAs per SM need the whole shared-memory carve-out
-    Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<NT, PAGED, NG>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+    Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<NT, PAGED, NG, ROWS>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
   return Q27B_OK;
 }
 
 }  // namespace
 
 int decode_ws_setup() {
-  if (int rc = ws_attr<1, false, 2>()) return rc;
-  if (int rc = ws_attr<2, false, 2>()) return rc;
-  if (int rc = ws_attr<3, false, 2>()) return rc;
-  if (int rc = ws_attr<1, true, 2>()) return rc;
-  if (int rc = ws_attr<2, true, 2>()) return rc;
-  if (int rc = ws_attr<3, true, 2>()) return rc;
-  if (int rc = ws_attr<1, true, 1>()) return rc;
-  if (int rc = ws_attr<2, true, 1>()) return rc;
-  if (int rc = ws_attr<3, true, 1>()) return rc;
+  if (int rc = ws_attr<1, false, 2, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<2, false, 2, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<3, false, 2, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<1, true, 2, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<2, true, 2, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<3, true, 2, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<1, true, 1, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<2, true, 1, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<3, true, 1, Rows::ALL>()) return rc;
+  if (int rc = ws_attr<1, false, 2, Rows::PREFIX>()) return rc;
+  if (int rc = ws_attr<2, false, 2, Rows::PREFIX>()) return rc;
+  if (int rc = ws_attr<3, false, 2, Rows::PREFIX>()) return rc;
+  if (int rc = ws_attr<1, true, 1, Rows::PREFIX>()) return rc;
+  if (int rc = ws_attr<2, true, 1, Rows::PREFIX>()) return rc;
+  if (int rc = ws_attr<3, true, 1, Rows::PREFIX>()) return rc;
   return Q27B_OK;
 }
 
-int launch_decode_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
-                     const DecodeParams& p, bool paged, int nseq, cudaStream_t s, WsGroups groups) {
+namespace {
+int setup_once() {
   static bool attr[64] = {};
   static std::mutex attr_mu;
   int dev;
   Q27B_CK(cudaGetDevice(&dev));
-  {
-    std::lock_guard<std::mutex> lock(attr_mu);
-    if (!attr[dev]) {
-      if (int rc = decode_ws_setup()) return rc;
-      attr[dev] = true;
-    }
+  std::lock_guard<std::mutex> lock(attr_mu);
+  if (!attr[dev]) {
+    if (int rc = decode_ws_setup()) return rc;
+    attr[dev] = true;
   }
-  const int nt = (GQA * p.T + 7) / 8;
-  if (groups != WsGroups::TWO && paged) {
-    const int smem = groups == WsGroups::SPREAD ? SPREAD_SMEM_BYTES : Lay<1>::SMEM_BYTES;
-    if (nt == 1) return launch_ws_nt<1, 1>(kv, ks, vv, vs, p, true, nseq, s, smem);
-    if (nt == 2) return launch_ws_nt<2, 1>(kv, ks, vv, vs, p, true, nseq, s, smem);
-    return launch_ws_nt<3, 1>(kv, ks, vv, vs, p, true, nseq, s, smem);
-  }
-  if (nt == 1) return launch_ws_nt<1, 2>(kv, ks, vv, vs, p, paged, nseq, s);
-  if (nt == 2) return launch_ws_nt<2, 2>(kv, ks, vv, vs, p, paged, nseq, s);
-  return launch_ws_nt<3, 2>(kv, ks, vv, vs, p, paged, nseq, s);
+  return Q27B_OK;
+}
+}  // namespace
+
+int launch_decode_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                     const DecodeParams& p, bool paged, int nseq, cudaStream_t s, WsGroups groups) {
+  if (int rc = setup_once()) return rc;
+  if (!paged) return launch_ws_t<false, 2, Rows::ALL>(kv, ks, vv, vs, p, nseq, s);
+  if (groups == WsGroups::TWO) return launch_ws_t<true, 2, Rows::ALL>(kv, ks, vv, vs, p, nseq, s);
+  return launch_ws_t<true, 1, Rows::ALL>(kv, ks, vv, vs, p, nseq, s, smem_of(groups));
+}
+
+int launch_prefix_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                     const DecodeParams& p, int nseq, cudaStream_t s) {
+  if (int rc = setup_once()) return rc;
+  return launch_ws_t<false, 2, Rows::PREFIX>(kv, ks, vv, vs, p, nseq, s);
+}
+int launch_prefix_ws_paged(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
+                           const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups) {
+  if (int rc = setup_once()) return rc;
+  return launch_ws_t<true, 1, Rows::PREFIX>(kv, ks, vv, vs, p, nseq, s, smem_of(groups));
 }
 
 int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
-                     const DecodeParams& p, int nseq, cudaStream_t s, WsGroups groups) {
+                     const ListParams& p, int nseq, cudaStream_t s, WsGroups groups) {
   static bool attr[64] = {};
   static std::mutex attr_mu;
   int dev;
@@ -914,10 +940,10 @@ int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtenso
   const dim3 grid(p.nch, p.nkvh, nseq);
   const bool paged = p.page_table != nullptr;
   if (groups == WsGroups::TWO) {
-    auto* k = paged ? decode_ws_kernel<1, true, 2, true> : decode_ws_kernel<1, false, 2, true>;
+    auto* k = paged ? decode_ws_kernel<1, true, 2, Rows::LIST> : decode_ws_kernel<1, false, 2, Rows::LIST>;
     Q27B_CK(launch_step(k, grid, dim3(Lay<2>::THREADS), Lay<2>::SEL_SMEM_BYTES, s, *kv, *ks, *vv, *vs, p));
   } else {
-    auto* k = paged ? decode_ws_kernel<1, true, 1, true> : decode_ws_kernel<1, false, 1, true>;
+    auto* k = paged ? decode_ws_kernel<1, true, 1, Rows::LIST> : decode_ws_kernel<1, false, 1, Rows::LIST>;
     const int smem = groups == WsGroups::SPREAD ? SPREAD_SMEM_BYTES : Lay<1>::SEL_SMEM_BYTES;
     Q27B_CK(launch_step(k, grid, dim3(Lay<1>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
   }

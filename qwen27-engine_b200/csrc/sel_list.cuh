@@ -7,13 +7,13 @@ namespace q27b {
 namespace {
 
 // Position of the token that grid slot z (sequence b, token t) stands for.
-__device__ __forceinline__ int sel_pos(const DecodeParams& p, bool paged, int z) {
+__device__ __forceinline__ int sel_pos(const ListParams& p, bool paged, int z) {
   return (paged ? p.seq_len[z / p.sel_T] - p.sel_T : *p.pos0) + z % p.sel_T;
 }
 
 // Entries [i0, i1) of the list of (z, kh) that have a row below n, in order, into `list` (shared memory); one warp, returns
 // how many. An entry that is no block, or whose page is none, is flagged and left out.
-__device__ __forceinline__ int collect_blocks(const DecodeParams& p, bool paged, int z, int kh, int i0, int i1, int n, int* list) {
+__device__ __forceinline__ int collect_blocks(const ListParams& p, bool paged, int z, int kh, int i0, int i1, int n, int* list) {
   const int lane = threadIdx.x & 31;
   const int* src = p.sel + ((size_t)z * p.nkvh + kh) * p.sel_k;
   int count = 0;
