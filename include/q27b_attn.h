@@ -448,7 +448,9 @@ int q27b_tree_plan(const int* parent, int T, uint64_t* mask, int* depth);
  * *pos0 + j for which bit j of mask[t] is set (its own only if bit t is; bits from T on are ignored); what the other rows
  * hold has no influence. Otherwise as q27b_attn_decode: GQA 6:1, softmax, o *= sigmoid(gate); a draft that sees nothing
  * gives 0. mask is device memory. Q * kq_scale, K, V and P are rounded to f16 for the tensor cores, sums are f32; the
- * output is therefore f16 (o: __half [T][nqh][256]) or, with xq != null, q8_1 as in q27b_attn_decode. */
+ * output is therefore f16 (o: __half [T][nqh][256]) or, with xq != null, q8_1 as in q27b_attn_decode. A V value of a draft that f16
+ * does not hold (infinite, NaN, or a q8_0 value times its scale from 65,520 on) is taken as it is, in f32, and meets its own
+ * dimension of the drafts that see it only; such a product in the prefix is infinite, as in q27b_attn_decode. */
 int q27b_attn_decode_tree(const float* qn, const float* qg, const void* kcache, const void* vcache, void* o, int8_t* xq,
                           float* xd, const int* pos0, const uint64_t* mask, int T, float kq_scale, int nqh, int nkvh,
                           int n_ctx, int q8, void* stream);

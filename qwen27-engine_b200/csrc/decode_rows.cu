@@ -37,13 +37,57 @@ __device__ __forceinline__ void write_row(const RowsParams& p, size_t row, int c
   if ((c & 7) == 0) p.xd[(row * AD + 4 * c) / 32] = __half2float(__float2half_rn(d));
 }
 
+// Dims 4 c .. 4 c + 3 of a row of head kh of a cache, in f32.
+__device__ __forceinline__ float4 four_of(const CacheRef& ref, const void* cache, int64_t at, int c) {
+  const uint8_t* base = (const uint8_t*)cache;
+  if (!ref.q8) {
+    const uint2 w = *(const uint2*)(base + at * 2 * AD + 8 * c);
+    const float2 lo = __half22float2(u32_as_h2(w.x)), hi = __half22float2(u32_as_h2(w.y));
+    return make_float4(lo.x, lo.y, hi.x, hi.y);
+  }
+  const uint32_t w = *(const uint32_t*)(base + at * AD + 4 * c);
+  const float d = __half2float(*(const __half*)(base + cache_rows(ref) * AD + at * 16 + (c >> 3) * 2));
+  return make_float4((float)(int8_t)w * d, (float)(int8_t)(w >> 8) * d, (float)(int8_t)(w >> 16) * d, (float)(int8_t)(w >> 24) * d);
+}
+
+// What the tree kernel leaves out of dims 4 c .. of a row: the V values, not finite in f16, of the drafts that the row sees, times
+// their weights relative to M. Rare, and kept out of line.
+__device__ __noinline__ float4 left_out(const RowsParams& p, size_t row, int c, float M) {
+  const int T = p.c.T, nqh = p.c.nkvh * GQA, b = (int)(row / ((size_t)T * nqh)), t = (int)(row / nqh % T), kh = (int)(row % nqh) / GQA;
+  uint64_t left = p.mask[(size_t)b * T + t];
+  if (T < 64) left &= ((uint64_t)1 << T) - 1;
+  float A[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (; left; left &= left - 1) {
+    const int64_t at = cache_row(p.c, b, kh, first_pos(p.c, b) + __ffsll((long long)left) - 1);
+    if (at < 0) continue;
+    const float4 v4 = four_of(p.c, p.vcache, at, c);
+    const float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) any |= !(fabsf(v[i]) < 65520.f);  // (from there on a value rounds to infinity in f16)
+    if (!any) continue;
+    float s = 0.f;
+#pragma unroll 1
+    for (int i = 0; i < AD / 4; i++) {
+      const float4 q = *(const float4*)(p.qn + row * AD + 4 * i), k = four_of(p.c, p.kcache, at, i);
+      s += q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
+    }
+    const float f = ex2((s * p.kq_scale - M) * LOG2E);
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      if (!(fabsf(v[i]) < 65520.f)) A[i] += f * v[i];
+  }
+  return make_float4(A[0], A[1], A[2], A[3]);
+}
+
 // Merges the partials of a row, applies the gate and writes f16, or q8_1; a row without a visible position is 0. 64 threads to
 // a row, four dims each, or four times as many that take every fourth partial; PRE partials of a thread are requested at a time, the
 // first before the maxima are known. 72 rows of 148 partials: PRE = 10 and two CTAs on an SM 18.4 us a call, 6 and three 20.1;
 // 384 rows of 49, which fill the SMs more than once with two CTAs: 29.0 and 26.4. Many rows have few partials each (a batch): a
 // CTA takes four rows then (6,144 rows of a few partials: 151.8 and 134.3 us a call, a CTA for every row 224).
-template <int GROUPS, int PRE, int CTAS>
-__global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams p, int64_t rows) {
+template <bool TREE, int GROUPS, int PRE, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const __grid_constant__ RowsParams p, int64_t rows) {
   constexpr int ROWS = 4 / GROUPS;  // of a CTA
   __shared__ float4 sa[GROUPS > 1 ? GROUPS - 1 : 1][64];
   __shared__ float sl[4], sm[8];
@@ -57,7 +101,7 @@ __global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams 
   float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
   if (mine) {
     g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c);
-    if (!p.sel) {
+    if (TREE) {
       b = (int)(row / ((size_t)p.c.T * nqh));
       const int h = (int)(row % nqh), gr = (int)(row / nqh % p.c.T) * GQA + h % GQA;
       y = gr / TREE_ROWS * p.c.nkvh + h / GQA;
@@ -69,7 +113,7 @@ __global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams 
   pdl_trigger();
   int np = 0;        // partials of the row: first, first + step, ..
   size_t first = 0, step = 1;
-  if (mine && p.sel) {
+  if (mine && !TREE) {
     np = p.nsplit;
     first = row * p.nsplit;
   } else if (mine && tiles > 0) {
@@ -111,10 +155,12 @@ __global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams 
   }
   float L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  uint32_t signs = 0;  // of the sums: the tree kernel left something out
   auto add = [&](const float2& v, const float4& x) {
+    if (TREE) signs |= __float_as_uint(v.y);
     if (v.y == 0.f) return;  // holds nothing
     const float f = ex2((v.x - M) * LOG2E);
-    L += v.y * f;
+    L += (TREE ? fabsf(v.y) : v.y) * f;
     A.x += x.x * f, A.y += x.y * f, A.z += x.z * f, A.w += x.w * f;
   };
   for (int z0 = grp; z0 < np; z0 += GROUPS * PRE) {
@@ -125,17 +171,22 @@ __global__ void __launch_bounds__(256, CTAS) rows_merge_kernel(const RowsParams 
   }
   if (GROUPS > 1) {
     if (grp > 0) sa[grp - 1][c] = A;
-    if (c == 0) sl[grp] = L;
+    if (c == 0) sl[grp] = TREE ? __uint_as_float(__float_as_uint(L) | (signs & 0x80000000u)) : L;
     __syncthreads();
     if (grp > 0) return;
 #pragma unroll
     for (int k = 0; k < GROUPS - 1; k++) {
       const float4 x = sa[k][c];
       A.x += x.x, A.y += x.y, A.z += x.z, A.w += x.w;
-      L += sl[k + 1];
+      L += TREE ? fabsf(sl[k + 1]) : sl[k + 1];
+      if (TREE) signs |= __float_as_uint(sl[k + 1]);
     }
   }
   if (!mine) return;
+  if (TREE && signs >> 31) {
+    const float4 x = left_out(p, row, c, M);
+    A.x += x.x, A.y += x.y, A.z += x.z, A.w += x.w;
+  }
   write_row(p, row, c, A, L, g);
 }
 
@@ -156,17 +207,6 @@ __global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams
   const int first = first_pos(p.c, b), n = max(0, min(first, p.c.n_ctx));  // drafts, prefix
   const float4 g = *(const float4*)(p.qg + row * 2 * AD + AD + 4 * c), q = *(const float4*)(p.qn + row * AD + 4 * c);
   const uint64_t mask = p.mask[(size_t)b * T + t];
-  auto four = [&](const void* cache, int64_t at) {
-    const uint8_t* base = (const uint8_t*)cache;
-    if (!p.c.q8) {
-      const uint2 w = *(const uint2*)(base + at * 2 * AD + 8 * c);
-      const float2 lo = __half22float2(u32_as_h2(w.x)), hi = __half22float2(u32_as_h2(w.y));
-      return make_float4(lo.x, lo.y, hi.x, hi.y);
-    }
-    const uint32_t w = *(const uint32_t*)(base + at * AD + 4 * c);
-    const float d = __half2float(*(const __half*)(base + cache_rows(p.c) * AD + at * 16 + (c >> 3) * 2));
-    return make_float4((float)(int8_t)w * d, (float)(int8_t)(w >> 8) * d, (float)(int8_t)(w >> 16) * d, (float)(int8_t)(w >> 24) * d);
-  };
   float4 k[DRAFTS], v[DRAFTS];
   bool seen[DRAFTS];
 #pragma unroll
@@ -175,7 +215,7 @@ __global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams
     const int64_t at = j < T && ((mask >> j) & 1) ? cache_row(p.c, b, kh, first + j) : -1;
     k[d] = v[d] = make_float4(0.f, 0.f, 0.f, 0.f);
     seen[d] = at >= 0;
-    if (seen[d]) k[d] = four(p.kcache, at), v[d] = four(p.vcache, at);
+    if (seen[d]) k[d] = four_of(p.c, p.kcache, at, c), v[d] = four_of(p.c, p.vcache, at, c);
   }
 #pragma unroll
   for (int d = 0; d < DRAFTS; d++) {
@@ -249,9 +289,11 @@ __global__ void __launch_bounds__(256, CTAS) draft_merge_kernel(const RowsParams
   write_row(p, row, c, A, L, g);
 }
 
+template <bool TREE>
 int launch_rows_merge(const RowsParams& p, int64_t rows, int n_sm, cudaStream_t s) {
   const bool split = rows < 8 * (int64_t)n_sm;  // a row's partials among the groups of a CTA
-  auto* k = !split ? rows_merge_kernel<1, 6, 3> : rows > 2 * (int64_t)n_sm ? rows_merge_kernel<4, 6, 3> : rows_merge_kernel<4, 10, 2>;
+  auto* k = !split ? rows_merge_kernel<TREE, 1, 6, 3>
+            : rows > 2 * (int64_t)n_sm ? rows_merge_kernel<TREE, 4, 6, 3> : rows_merge_kernel<TREE, 4, 10, 2>;
   Q27B_CK(launch_step(k, dim3((unsigned)(split ? rows : (rows + 3) / 4)), dim3(256), 0, s, p, rows));
   return Q27B_OK;
 }
@@ -330,7 +372,7 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
     if (int rc = cached_tmap_2d(&vv, p.vcache, cache, 2 * AD, 2 * AD, 128, BLK, true)) return rc;
     if (int rc = launch_blocks_f16(&kv, &vv, d, c.B * c.T, s)) return rc;
   }
-  return launch_rows_merge(p, rows, ctx->n_sm, s);
+  return launch_rows_merge<false>(p, rows, ctx->n_sm, s);
 }
 
 int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
@@ -373,7 +415,7 @@ int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   p.part_o = part + head;
   p.part_ml = (float2*)(p.part_o + slots * TREE_ROWS * AD);
   if (int rc = launch_tree(p, ctx->n_sm, s)) return rc;
-  return launch_rows_merge(p, rows, ctx->n_sm, s);
+  return launch_rows_merge<true>(p, rows, ctx->n_sm, s);
 }
 
 }  // namespace

@@ -22,7 +22,7 @@ struct RowsParams {
   int k;
   float kq_scale;
   float* part_o;         // unnormalised O of a row of a part, 256 floats each: [row][nsplit] (blocks) or [part][128 rows] (tree)
-  float2* part_ml;       // (max, sum) of the same
+  float2* part_ml;       // (max, sum) of the same; tree: the sum's sign is set where V values of drafts are left to the merge
   int nsplit;            // parts of a list, or of a row tile of one sequence
   int64_t* plan;         // tree, paged: [0] tiles of a part, [1 + b] parts of a unit summed over the sequences before b (tree_parts)
 };

@@ -11,8 +11,9 @@
 // (tree_share), and finds its own part. A tile that reaches into
 // the drafted rows gets a 64-bit word of visible columns per row: the row's mask, shifted to the tile.
 // Weights of columns that a row does not see are 0, and so that 0 times what lies there is 0, V rows that no row
-// may see (past the sequence, on a page that does not exist) are cleared on the way to the tensor core, and drafted V
-// chunks of 16 dims that are not finite are cleared and remembered: the rows that see such a draft get NaN in these dims.
+// may see (past the sequence, on a page that does not exist) are cleared on the way to the tensor core, and so are drafted V
+// values that are not finite in f16: the rows that see such a draft say so with the sign of their sum, and the merge adds weight times
+// value to them in f32.
 //
 // Warps 0-3 softmax of the even tiles and 4-7 of the odd ones, a thread a row; warp 8 issues the Q K^T MMAs, warp 9 the P V MMAs.
 // f16 cache: warp 10 brings the tiles by TMA as the tensor core reads them. q8_0 cache: warps 10-13 turn K and 14-17 V into f16
@@ -48,8 +49,8 @@ constexpr int OFF_V = OFF_K + NK * KV_BYTES;
 constexpr int OFF_STAGE = OFF_V + NV * KV_BYTES;          // the Q tile on its way to tensor memory, 2 KB a softmax warp
 constexpr int OFF_XCH = OFF_STAGE + NSW * 2048;           // f32: [128] reference maxima, [NWG][128] sums
 constexpr int OFF_BAR = OFF_XCH + (1 + NWG) * QT * 4;
-constexpr int OFF_BAD = OFF_BAR + NBAR * 8;               // [16 chunks of 16 dims][2 words]: drafts whose V chunk is not finite
-constexpr int OFF_SKIP = OFF_BAD + 16 * 8;                // [TREE_MAX_TILES / 32] words: tiles on pages that do not exist
+constexpr int OFF_BAD = OFF_BAR + NBAR * 8;               // [2 words]: drafts of whose V rows something was cleared
+constexpr int OFF_SKIP = OFF_BAD + 8;                     // [TREE_MAX_TILES / 32] words: tiles on pages that do not exist
 constexpr int OFF_SCAN = OFF_SKIP + TREE_MAX_TILES / 8;   // [32] 64-bit sums
 constexpr int OFF_MISC = OFF_SCAN + 32 * 8;
 constexpr int SMEM_BYTES = OFF_MISC + 16 + 1024;
@@ -73,23 +74,25 @@ __device__ __forceinline__ void ref_wait(int q, int parity) { asm volatile("bar.
 __device__ __forceinline__ void row_sync(int q) { asm volatile("bar.sync %0, %1;" ::"r"(9 + q), "n"(64) : "memory"); }
 __device__ __forceinline__ bool not_finite(uint32_t h2) { return (h2 & 0x7C00u) == 0x7C00u || (h2 & 0x7C000000u) == 0x7C000000u; }
 
-// Clears the 16-byte chunks of a swizzled f16 V tile that may not reach the tensor core: position p (row r of the tile),
-// dims 64 sg .. 64 sg + 63. Rows from `end` on go entirely; chunks of drafted rows (from `zone` on) that are not finite go
-// and are noted in bad[chunk of 16 dims][draft].
-__device__ __noinline__ void clean_v_row(uint8_t* vrow, int r, int sg, int zone, int end, int draft, uint32_t* bad) {
-#pragma unroll 1
-  for (int c = 0; c < 8; c++) {
-    uint4* at = (uint4*)(vrow + ((c ^ (r & 7)) << 4));
-    if (r >= end) {
-      *at = make_uint4(0, 0, 0, 0);
-    } else if (r >= zone) {
-      const uint4 x = *at;
-      if (not_finite(x.x) || not_finite(x.y) || not_finite(x.z) || not_finite(x.w)) {
-        *at = make_uint4(0, 0, 0, 0);
-        atomicOr(&bad[2 * (4 * sg + c / 2) + (draft >> 5)], 1u << (draft & 31));
-      }
-    }
-  }
+__device__ __forceinline__ uint32_t finite_of(uint32_t h2) {  // 0 for a half that is none
+  return h2 & (((h2 & 0x7C00u) == 0x7C00u ? 0u : 0xFFFFu) | ((h2 & 0x7C000000u) == 0x7C000000u ? 0u : 0xFFFF0000u));
+}
+
+// Clears what may not reach the tensor core of row r of a swizzled f16 V tile, dims 64 sg .. 64 sg + 63: all of a row that no draft
+// has (draft < 0), else the values that are not finite, noted in bad[draft].
+__device__ __forceinline__ void clean_v_row(uint8_t* vrow, int r, int draft, uint32_t* bad) {
+  uint4 x[8];
+  bool odd = draft < 0;
+#pragma unroll
+  for (int c = 0; c < 8; c++) x[c] = *(const uint4*)(vrow + ((c ^ (r & 7)) << 4));
+#pragma unroll
+  for (int c = 0; c < 8; c++) odd |= not_finite(x[c].x) || not_finite(x[c].y) || not_finite(x[c].z) || not_finite(x[c].w);
+  if (!odd) return;
+  if (draft >= 0) atomicOr(&bad[draft >> 5], 1u << (draft & 31));
+#pragma unroll
+  for (int c = 0; c < 8; c++)
+    *(uint4*)(vrow + ((c ^ (r & 7)) << 4)) =
+        draft < 0 ? make_uint4(0, 0, 0, 0) : make_uint4(finite_of(x[c].x), finite_of(x[c].y), finite_of(x[c].z), finite_of(x[c].w));
 }
 
 // 16 bytes of the cache, read once.
@@ -208,10 +211,10 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       mbar_init(&bar[B_PFULL + s], n_active);
       mbar_init(&bar[B_PVDONE + s], 1);
     }
-    mbar_init(&bar[B_ODONE], 1);
+    mbar_init(&bar[B_ODONE], 2);
     mbar_fence_init();
   }
-  if (tid < 32) bad[tid] = 0;
+  if (tid < 2) bad[tid] = 0;
   if (PAGED) {  // the pages of this part: what lies on one that is none is not visible
     for (int j = tid; j < (nt + 31) / 32; j += THREADS) skip[j] = 0;
     __syncthreads();
@@ -364,12 +367,13 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
         }
         tmem_st16(tlane + TM_S + wg * PT + 16 * half, w);  // over the scores that it was made of
       }
-      if (!Q8 && p_tile + PT > zone) {  // f16 cache: V lies in the operand buffer as it came (the converters do this for q8_0)
-        const int vb = j % NV;
+      if (!Q8 && p_tile + PT > zone) {  // rows of drafts, and, as they came, rows behind the sequence (q8_0: the P V issuer sees to them)
+        const int vb = j % NV, r0 = max(0, zone - p_tile);
         mbar_wait(&bar[B_VFULL + vb], (j / NV) & 1, abort_flag, p.c.status);
         for (int u = q * 32 + lane; u < 4 * PT; u += 32 * n_active)  // (segment, row)
-          clean_v_row(sgen + OFF_V + vb * KV_BYTES + (u >> 6) * SEGK + (u & 63) * 128, u & 63, u >> 6, zone - p_tile, n_end - p_tile,
-                      p_tile + (u & 63) - first, bad);
+          if ((u & 63) >= r0)
+            clean_v_row(sgen + OFF_V + vb * KV_BYTES + (u >> 6) * SEGK + (u & 63) * 128, u & 63,
+                        p_tile + (u & 63) < n_end ? p_tile + (u & 63) - first : -1, bad);
       }
       if (!Q8) fence_proxy_async();
       tc_wait_st();
@@ -387,8 +391,11 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     xch[(1 + wg) * QT + r] = l;
     row_sync(q);
     l += xch[(1 + (wg ^ 1)) * QT + r];
-    if (wg == 0 && t < T) p.part_ml[slot0 + r] = make_float2(m_ref, l);
     mbar_wait(&bar[B_ODONE], 0, abort_flag, p.c.status);
+    if (wg == 0 && t < T) {
+      if (((uint64_t)bad[0] | (uint64_t)bad[1] << 32) & mine) l = __uint_as_float(__float_as_uint(l) | 0x80000000u);
+      p.part_ml[slot0 + r] = make_float2(m_ref, l);
+    }
     tc_fence_after();
     // 32 columns at a time through shared memory (the K buffers are free now): TMEM gives a thread a row, and a row per
     // thread would touch 32 lines with every store; read back, eight lanes share 128 contiguous bytes of a row.
@@ -400,13 +407,6 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
         uint32_t v[32];
         tmem_ld32(tlane + TM_O + d0, v);
         tc_wait_ld();
-#pragma unroll
-        for (int h = 0; h < 2; h++) {  // chunks of 16 dims in which a draft that this row sees is not finite
-          const uint64_t nf = (uint64_t)bad[2 * (d0 / 16 + h)] | (uint64_t)bad[2 * (d0 / 16 + h) + 1] << 32;
-          if (nf & mine)
-#pragma unroll
-            for (int i = 0; i < 16; i++) v[16 * h + i] = 0x7FFFFFFFu;
-        }
 #pragma unroll
         for (int i = 0; i < 8; i++) *(uint4*)(stage + swz128(lane, i)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
       }
@@ -450,9 +450,19 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
     int st = 0, ph = 0;  // V buffer and its phase
 #pragma unroll 1
     for (int j = 0; j < nt; j++) {
-      const int pb = j & 1;
-      mbar_wait(&bar[B_PFULL + pb], (j >> 1) & 1, abort_flag, p.c.status);
+      const int pb = j & 1, p_tile = (it0 + j) * PT;
       mbar_wait(&bar[B_VFULL + st], ph, abort_flag, p.c.status);
+      if (Q8 && p_tile + PT > zone) {  // rows of drafts, while the softmax warps are at this tile
+        const int r0 = max(0, zone - p_tile), rows = min(PT, n_end - p_tile) - r0;
+#pragma unroll 1
+        for (int u = lane; u < 4 * rows; u += 32) {  // (segment, row): neighbouring lanes on neighbouring rows have no bank conflicts
+          const int vr = r0 + u % rows;
+          clean_v_row(sgen + OFF_V + st * KV_BYTES + u / rows * SEGK + vr * 128, vr, p_tile + vr - first, bad);
+        }
+        fence_proxy_async();
+        __syncwarp();
+      }
+      mbar_wait(&bar[B_PFULL + pb], (j >> 1) & 1, abort_flag, p.c.status);
       tc_fence_after();
       if (issuer) {
 #pragma unroll
@@ -466,6 +476,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       __syncwarp();
       if (++st == NV) st = 0, ph ^= 1;
     }
+    if (lane == 0) mbar_arrive(&bar[B_ODONE]);  // with it `bad` is there
   } else if constexpr (!Q8) {
     // ================================================================ TMA producer (f16 cache)
     if (lane == 0) {
@@ -518,7 +529,7 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       d[k] = whole || 8 * k < there ? *(const uint16_t*)(ssrc + r * 16) : 0;
     };
     // Item k of the tile in registers into the f16 buffer, and the same item of the next tile fetched in its place.
-    auto convert = [&](int k, uint8_t* dst, bool more, bool whole, int drafted) {
+    auto convert = [&](int k, uint8_t* dst, bool more, bool whole) {
       const __half2 dd = u32_as_h2(__byte_perm(d[k], d[k], 0x1010));
       const uint32_t xw[4] = {x[k].x ^ 0x80808080u, x[k].y ^ 0x80808080u, x[k].z ^ 0x80808080u, x[k].w ^ 0x80808080u};
       uint32_t o[8];
@@ -528,16 +539,6 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
         o[2 * w + 1] = dq_pair(__byte_perm(xw[w], 0x64646464u, 0x4342), dd);
       }
       if (more) fetch(k, whole);
-      if (drafted >= 0) {  // this row is a draft's
-        bool nf = false;
-#pragma unroll
-        for (int w = 0; w < 8; w++) nf |= not_finite(o[w]);
-        if (nf) {
-          atomicOr(&bad[2 * c16 + (drafted >> 5)], 1u << (drafted & 31));
-#pragma unroll
-          for (int w = 0; w < 8; w++) o[w] = 0;
-        }
-      }
       *(uint4*)(dst + a.dst + k * 1024) = make_uint4(o[0], o[1], o[2], o[3]);
       *(uint4*)(dst + (a.dst ^ 16u) + k * 1024) = make_uint4(o[4], o[5], o[6], o[7]);
     };
@@ -553,15 +554,12 @@ tree_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CU
       if (more) aim(j + 1);
       mbar_wait(&bar[b_empty + fb], ph, abort_flag, p.c.status);  // the MMAs of the tile before it have read the buffer
       uint8_t* dst = sgen + (is_v ? OFF_V : OFF_K) + fb * KV_BYTES;
-      if (more && tile_rows(j + 1) == PT && p_tile + PT <= zone) {
+      if (more && tile_rows(j + 1) == PT) {
 #pragma unroll
-        for (int k = 0; k < 8; k++) convert(k, dst, true, true, -1);
+        for (int k = 0; k < 8; k++) convert(k, dst, true, true);
       } else {
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-          const int pos = p_tile + a.row0 + 8 * k;
-          convert(k, dst, more, false, is_v && pos >= zone && pos < n_end ? pos - first : -1);
-        }
+        for (int k = 0; k < 8; k++) convert(k, dst, more, false);
       }
       fence_proxy_async();
       __syncwarp();
