@@ -436,8 +436,8 @@ int q27b_prefill_qk_debug(const float* x, int rows, float kq_scale, const void* 
  * parts, or Q27B_UNSUPPORTED) or, for trees of up to four drafts, in the decode buffer; over pages in the paged buffer. Calls
  * that can overlap on the GPU race on it, so keep those of one device in one stream order. Float and cache pointers lie on
  * 16-byte boundaries. Indices that the device finds out of range are reported in the device status word (bit 1: page table,
- * bit 2: path or list of blocks) and nothing is read or written there: a path's or list's entry is skipped, the rows of a
- * page are skipped or, for trees of up to four drafts as in q27b_attn_decode_paged, stand for those of page 0. */
+ * bit 2: path or list of blocks) and nothing is read or written there: a path's or list's entry is skipped, and so are the rows
+ * of a page (q27b_attn_decode_paged takes those of page 0 in their place). */
 
 /* Masks and depths of a tree of T = 1..64 drafts in which parent[t] is the draft before t (smaller than t) or -1 for a
  * child of the last accepted token: mask[t] has bit j set for j = t and every ancestor j of t, depth[t] (may be null)

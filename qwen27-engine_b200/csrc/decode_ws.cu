@@ -64,6 +64,7 @@ constexpr int P_WORDS = MAXR * P_STRIDE;
 constexpr int Q_STRIDE = 2 * AD + 16;             // bytes per staged Q row (f16; 16 bytes of padding: conflict-free 16-byte reads)
 constexpr int SCHED_DONE = 32;                    // p.sched: [KV head] pool counters, [32] CTAs that are done
 constexpr float TAU = 8.0f;                       // a score may exceed the reference max by this much
+constexpr int ABSENT = 1 << 24;                   // PREFIX: number of a tile whose page is none (behind every sequence: nothing of it is seen)
 constexpr int O_XCH_BYTES = 128 * 12 * 16;        // end-of-kernel O exchange: [12][128 threads] float4, the accumulators of half a thread
 
 // Shared memory map of a CTA with NG tile groups (offsets from a 1024-byte aligned base). NG = 2: the
@@ -267,13 +268,14 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
 
   // Row of the K/V tensors at which tile t starts.
   auto tile_row = [&](int t) {
+    if (ROWS == Rows::PREFIX && PAGED && t == ABSENT) return kh * Q27B_PAGE;  // rows that are there, to no effect
     int row = kh * p.n_ctx + t * TILE;
     if (PAGED) {  // a tile never straddles a page (64 | 256)
       const int pp = t * TILE;
       int owner = seq;
       if constexpr (SEL) owner = seq / p.sel_T;
       int pg = p.page_table[(size_t)owner * p.max_pages + pp / Q27B_PAGE];
-      if (pg < 0 || pg >= p.n_pages) {  // never read outside the pool: flag it and read page 0
+      if (ROWS != Rows::PREFIX && (pg < 0 || pg >= p.n_pages)) {  // never read outside the pool: flag it and read page 0 (PREFIX: next_tile)
         atomicOr(p.status, ST_BAD_PAGE);
         pg = 0;
       }
@@ -307,6 +309,13 @@ decode_ws_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constan
   auto next_tile = [&](int j) {
     const int i = grp + NG * j;
     if (SEL) return i < n_static ? list[i] : -1;
+    if (ROWS == Rows::PREFIX && PAGED && i < n_static) {
+      const int pg = p.page_table[(size_t)seq * p.max_pages + (t_first + i) * TILE / Q27B_PAGE];
+      if (pg < 0 || pg >= p.n_pages) {
+        atomicOr(p.status, ST_BAD_PAGE);
+        return ABSENT;
+      }
+    }
     if (i < n_static) return t_first + i;
     if (!has_pool) return -1;
     const int t = pool0 + atomicAdd(p.sched + kh, 1);

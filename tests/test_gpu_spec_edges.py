@@ -64,3 +64,61 @@ def test_one_infinite_value_stays_in_its_dim(q27, T, paged, q8, n_ctx):
     assert torch.equal(o == math.inf, y == math.inf) and torch.equal(o == -math.inf, y == -math.inf)
     close(o, (*ref[:3], inv), torch.isfinite(y))
     assert q27.device_status() == 0
+
+
+# ---------------------------------------------------------------- pages that do not exist
+@pytest.mark.parametrize("T", [1, 3, 4, 5, 30])
+@pytest.mark.parametrize("where", ["first", "middle", "prefix end", "drafts"])
+def test_rows_of_a_page_that_does_not_exist_are_not_seen(q27, T, where):
+    """Every sequence of the batch has its result: the one with the bad page that of the other pages' rows alone."""
+    lens = [1100, 300 + T, 2000]
+    st = H.Store(lens, T, 2, True, True, seed=T)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    masks = H.random_masks(3, T, seed=T)
+    qn, qg = H.queries(st, 3)
+    b = 2
+    page = {"first": 0, "middle": 3, "prefix end": (lens[b] - T - 1) // 256, "drafts": (lens[b] - 1) // 256}[where]
+    whole = H.tree_visible(st, masks)
+    ref = H.attention(st, kc, vc, qn, qg, lambda s, t, h: [p for p in whole(s, t, h) if s != b or p // 256 != page])
+    for bad in (-1, st.n_pages, 2 ** 31 - 1, -2 ** 31):
+        st.table[b, page] = bad
+        o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+        assert q27.device_status() == 2
+        H.check_attention(o, ref)
+
+
+def test_no_page_at_all(q27):
+    for T in (2, 7):
+        st = H.Store([700], T, 2, True, True, seed=T)
+        kc, vc = st.new(), st.new()
+        st.fill(kc, H.gen(1))
+        st.fill(vc, H.gen(2))
+        st.table.fill_(-1)
+        qn, qg = H.queries(st, 3)
+        o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(H.random_masks(1, T, seed=1)))
+        assert (o == 0).all() and q27.device_status() == 2
+
+
+@pytest.mark.parametrize("page", [0, 2, 7])
+def test_blocks_of_a_page_that_does_not_exist_are_not_seen(q27, page):
+    lens, T, k = [2000, 500], 2, 12
+    st = H.Store(lens, T, 2, True, True, seed=1)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    qn, qg = H.queries(st, 3)
+    r = random.Random(page)
+    sel = torch.tensor([[[sorted(r.sample(range(-(-n // 64)), min(k, -(-n // 64)))) + [-1] * (k - min(k, -(-n // 64))) for _ in range(2)]
+                         for _ in range(T)] for n in lens], dtype=torch.int32)
+    sel[0, :, :, 0] = 4 * page
+
+    def visible(b, t, h):
+        last = lens[b] - T + t
+        return [p for x in sel[b, t, h].tolist() if x >= 0 and not (b == 0 and x // 4 == page) for p in range(64 * x, min(64 * x + 64, last + 1))]
+    ref = H.attention(st, kc, vc, qn, qg, visible)
+    st.table[0, page] = st.n_pages
+    o = H.call_blocks(q27, st, kc, vc, qn, qg, sel.cuda())
+    assert q27.device_status() == 2
+    H.check_attention(o, ref)
