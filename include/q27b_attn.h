@@ -57,8 +57,8 @@ int q27b_device_status(int* status_out);
 
 /* The per-device workspace (the counterpart of the reference's static AttnWs ws[16] and pbuf[16],
  * src/attn.cu:869-879,954-959), for callers that want control. All three act on the current device.
- *  - query: bytes currently held for the decode partials, the prefill partials and the paged-decode
- *    partials (0 = not allocated yet), and whether the workspace has been fixed.
+ *  - query: bytes currently held for the decode partials, the prefill partials and the calls over pages,
+ *    outgrown buffers among the latter (0 = not allocated yet), and whether the workspace has been fixed.
  *  - init: allocates everything now - the decode partials, the prefill partials at prefill_bytes
  *    (0: the default cap of 128 MiB) and paged_bytes for the batched paged decode (0: none) - and
  *    fixes it: afterwards no entry point allocates or frees device memory (q27b_attn_decode_ref

@@ -63,15 +63,22 @@ namespace {
 // tile on the split path, 2 x 2048 x 24 rows = 101 MB. (The reference fixes 24 MB on a 16 GB card.)
 constexpr size_t PF_CAP_DEFAULT_FLOATS = (128ull << 20) / sizeof(float);
 
+int frozen_ws(const char* what, size_t have, size_t need) {
+  return fail(Q27B_UNSUPPORTED, std::string(what) + ": the workspace was fixed by q27b_attn_workspace_init and holds " +
+                                    std::to_string(have * sizeof(float)) + " bytes, this call needs " + std::to_string(need * sizeof(float)));
+}
+int alloc_floats(size_t floats, float** p) {
+  const cudaError_t e = cudaMalloc(p, floats * sizeof(float));
+  if (e == cudaErrorMemoryAllocation) (void)cudaGetLastError();  // nothing is wrong with the device: no later call shall find this error
+  Q27B_CK(e);
+  return Q27B_OK;
+}
 int alloc_ws(DeviceCtx* ctx, WsBuf* b, size_t floats, const char* what) {
-  if (ctx->frozen)
-    return fail(Q27B_UNSUPPORTED, std::string(what) + ": the workspace was fixed by q27b_attn_workspace_init and holds " +
-                                      std::to_string(b->floats * sizeof(float)) + " bytes, this call needs " +
-                                      std::to_string(floats * sizeof(float)));
+  if (ctx->frozen) return frozen_ws(what, b->floats, floats);
   if (b->p) Q27B_CK(cudaFree(b->p));
   b->p = nullptr;
   b->floats = 0;
-  Q27B_CK(cudaMalloc(&b->p, floats * sizeof(float)));
+  if (int rc = alloc_floats(floats, &b->p)) return rc;
   b->floats = floats;
   return Q27B_OK;
 }
@@ -95,21 +102,14 @@ int prefill_ws(DeviceCtx* ctx, float** out, size_t* max_floats) {
   return Q27B_OK;
 }
 
-int paged_ws(DeviceCtx* ctx, size_t floats, float** out, const char* who) {
-  if (ctx->paged.floats < floats) {
-    WsBuf next;
-    if (!ctx->frozen) floats = std::max(floats, ctx->paged.floats + ctx->paged.floats / 2);
-    else next.floats = ctx->paged.floats;  // (for the message)
-    try {
-      ctx->outgrown.reserve(ctx->outgrown.size() + 1);
-    } catch (const std::exception&) {
-      return fail(Q27B_CUDA_ERROR, std::string(who) + ": out of host memory");
-    }
-    if (int rc = alloc_ws(ctx, &next, floats, who)) return rc;
-    if (ctx->paged.p) ctx->outgrown.push_back(ctx->paged.p);
-    ctx->paged = next;
+int paged_ws(DeviceCtx* ctx, size_t floats, float** out, const char* who, bool spare) {
+  if (ctx->frozen && ctx->paged.live.floats < floats) return frozen_ws(who, ctx->paged.live.floats, floats);
+  try {
+    if (int rc = ctx->paged.reserve(floats, spare, alloc_floats)) return rc;
+  } catch (const std::bad_alloc&) {
+    return fail(Q27B_CUDA_ERROR, std::string(who) + ": out of host memory");
   }
-  *out = ctx->paged.p;
+  *out = ctx->paged.live.p;
   return Q27B_OK;
 }
 
@@ -248,7 +248,7 @@ int q27b_attn_workspace_query(uint64_t* decode_bytes, uint64_t* prefill_bytes, u
   if (int rc = device_ctx(&ctx)) return rc;
   if (decode_bytes) *decode_bytes = ctx->dec.floats * sizeof(float);
   if (prefill_bytes) *prefill_bytes = ctx->pf.floats * sizeof(float);
-  if (paged_bytes) *paged_bytes = ctx->paged.floats * sizeof(float);
+  if (paged_bytes) *paged_bytes = ctx->paged.floats_held() * sizeof(float);
   if (fixed) *fixed = ctx->frozen ? 1 : 0;
   return Q27B_OK;
 }
@@ -265,7 +265,7 @@ int q27b_attn_workspace_init(uint64_t prefill_bytes, uint64_t paged_bytes) {
   if (int rc = decode_ws(ctx, &dummy)) return rc;
   if (int rc = prefill_ws(ctx, &dummy, &cap)) return rc;
   if (paged_bytes)
-    if (int rc = paged_ws(ctx, (size_t)((paged_bytes + sizeof(float) - 1) / sizeof(float)), &dummy)) return rc;
+    if (int rc = paged_ws(ctx, (size_t)((paged_bytes + sizeof(float) - 1) / sizeof(float)), &dummy, "attn_workspace_init", false)) return rc;
   ctx->frozen = true;
   return Q27B_OK;
 }
@@ -274,13 +274,13 @@ int q27b_attn_workspace_destroy(void) {
   DeviceCtx* ctx;
   if (int rc = device_ctx(&ctx)) return rc;
   Q27B_CK(cudaDeviceSynchronize());
-  for (WsBuf* b : {&ctx->dec, &ctx->pf, &ctx->paged}) {
+  for (WsBuf* b : {&ctx->dec, &ctx->pf, &ctx->paged.live}) {
     if (b->p) Q27B_CK(cudaFree(b->p));
     b->p = nullptr;
     b->floats = 0;
   }
-  for (float* p : ctx->outgrown) Q27B_CK(cudaFree(p));
-  ctx->outgrown.clear();
+  for (const WsBuf& b : ctx->paged.outgrown) Q27B_CK(cudaFree(b.p));
+  ctx->paged.outgrown.clear();
   if (ctx->ref_scores) Q27B_CK(cudaFree(ctx->ref_scores));
   ctx->ref_scores = nullptr;
   ctx->ref_scores_floats = 0;

@@ -8,9 +8,9 @@
 #include <cstdint>
 #include <initializer_list>
 #include <string>
-#include <vector>
 
 #include "../../include/q27b_attn.h"
+#include "ws_buf.h"
 
 namespace q27b {
 
@@ -27,13 +27,6 @@ const char* g_err_text();
                                                cudaGetErrorString(e_));                                    \
   } while (0)
 
-// One per-device workspace buffer. cap_floats > 0: the size it is allocated with on first use and
-// never exceeds (a call that would need more fails or splits less).
-struct WsBuf {
-  float* p = nullptr;
-  size_t floats = 0;
-};
-
 struct DeviceCtx {
   int dev = -1;
   int n_sm = 0;
@@ -42,8 +35,7 @@ struct DeviceCtx {
   // names (the reference keeps its prefill buffer apart and fixed for the same reason, src/attn.cu:954-959):
   WsBuf dec;                  // decode of one sequence: n_sm chunk partials, fixed size, allocated on first use
   WsBuf pf;                   // prefill: allocated once at pf_cap_floats; the split count is cut to fit
-  WsBuf paged;                // calls over pages: grows with the batch unless the workspace is frozen
-  std::vector<float*> outgrown;  // what `paged` was before: captured graphs may name it, so it stays until the workspace is destroyed
+  GrowingWs paged;            // calls over pages: grows with the batch unless the workspace is frozen
   size_t pf_cap_floats = 0;   // 0: default (see workspace_defaults in host.cu)
   bool frozen = false;        // after q27b_attn_workspace_init: nothing may be allocated any more
   float* ref_scores = nullptr;  // scratch of the slow checking kernel (q27b_attn_decode_ref), grown on demand
@@ -61,9 +53,9 @@ int device_ctx(DeviceCtx** out);
 int decode_ws(DeviceCtx* ctx, float** out);
 // The prefill partial buffer, allocated once at its cap. *max_floats = its size.
 int prefill_ws(DeviceCtx* ctx, float** out, size_t* max_floats);
-// The buffer of the calls over pages with room for `floats`; grows when it has to (to half as much again at least; the old one
-// stays allocated), unless the workspace is frozen, in which case a larger request of `who` fails with Q27B_UNSUPPORTED.
-int paged_ws(DeviceCtx* ctx, size_t floats, float** out, const char* who = "attn_decode_paged");
+// The buffer of the calls over pages with room for `floats`; grows when it has to (GrowingWs; spare: with room for more), unless
+// the workspace is frozen, in which case a larger request of `who` fails with Q27B_UNSUPPORTED.
+int paged_ws(DeviceCtx* ctx, size_t floats, float** out, const char* who = "attn_decode_paged", bool spare = true);
 // Whether one of the addresses is not on a 16-byte boundary (null is): the kernels load and store 16 bytes at a time.
 inline bool misaligned(std::initializer_list<const void*> ptrs) {
   for (const void* p : ptrs)

@@ -122,3 +122,31 @@ def test_blocks_of_a_page_that_does_not_exist_are_not_seen(q27, page):
     o = H.call_blocks(q27, st, kc, vc, qn, qg, sel.cuda())
     assert q27.device_status() == 2
     H.check_attention(o, ref)
+
+
+# ---------------------------------------------------------------- workspace
+def test_the_query_counts_outgrown_buffers_and_a_fixed_size_is_exact(q27):
+    def step(lens, T):
+        st = H.Store(lens, T, 2, True, True, seed=1)
+        kc, vc = st.new(), st.new()
+        st.fill(kc, H.gen(1))
+        st.fill(vc, H.gen(2))
+        masks = H.random_masks(st.B, T, seed=1)
+        qn, qg = H.queries(st, 3)
+        o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+        H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+    try:
+        q27.workspace_destroy()
+        step([200], 2)
+        first = q27.workspace_query()[2]
+        step([200] * 3, 9)
+        both = q27.workspace_query()[2]
+        live = both - first
+        assert first > 0 and live >= first + first // 2
+        q27.workspace_init(0, live + 4096)
+        assert q27.workspace_query()[2:] == (both + live + 4096, True)
+        step([200] * 3, 9)
+    finally:
+        torch.cuda.synchronize()
+        q27.workspace_destroy()
+    assert q27.workspace_query() == (0, 0, 0, False)
