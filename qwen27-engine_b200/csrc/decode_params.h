@@ -52,9 +52,6 @@ __host__ __device__ inline int filled_chunks(int n, int nch) {
   return tiles < 1 ? 1 : (tiles + share - 1) / share;
 }
 
-// Entries of a list that a CTA takes at most.
-constexpr int SEL_CHUNK = 128;
-
 // Split-K decode over a q8_0 cache on the tcgen05 path (decode_tc.cu). Same grid, same partial
 // layout and same tensor maps as the warp-MMA kernel. paged: rows through the page table.
 int launch_decode_tc(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
@@ -74,10 +71,10 @@ int launch_prefix_ws_paged(const CUtensorMap* kv, const CUtensorMap* ks, const C
 // The same with the P V contraction on tcgen05 (decode_wt.cu).
 int launch_decode_wt(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
                      const DecodeParams& p, bool paged, int nseq, cudaStream_t s);
-// Decode over lists of blocks: the warp-specialised kernel (q8_0, p.page_table null: contiguous; groups as above) and the
-// single-role kernel of decode.cu (f16 caches). nseq = B * sel_T.
+// Decode over lists of blocks: the warp-specialised kernel (q8_0, p.page_table null: contiguous; pairs: CTAs of one tile group,
+// two to an SM, instead of two) and the single-role kernel of decode.cu (f16 caches). nseq = B * sel_T.
 int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
-                     const ListParams& p, int nseq, cudaStream_t s, WsGroups groups);
+                     const ListParams& p, int nseq, cudaStream_t s, bool pairs);
 int launch_blocks_f16(const CUtensorMap* kv, const CUtensorMap* vv, const ListParams& p, int nseq, cudaStream_t s);
 // The attention of T = 1..4 tokens to the rows before them alone, by the kernels of a decode call (q8_0: the warp-specialised one;
 // f16: decode.cu); partials [sequence][KV head][chunk][24][258].

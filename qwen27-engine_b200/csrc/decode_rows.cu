@@ -311,45 +311,13 @@ int place_partials(DeviceCtx* ctx, RowsParams& p, int64_t rows, int64_t more, in
 }
 int no_room(const char* who) { return fail(Q27B_UNSUPPORTED, std::string(who) + ": the prefill workspace is too small for the partials of this call"); }
 
-// How lists of k blocks are cut into chunks, a CTA each: the plan of the least time in a model of the launch (us). A round of CTAs
-// costs C0 and so much a block: an SM to itself for a CTA of two tile groups 0.71 (q8_0) or 1.1 (f16), for one of one group
-// 0.97, and 1.37 where two of those share it. Measured on 14 shapes (1 to 512 lists of 16 to 1,024 blocks): 4 lists of 128
-// blocks 11.7 us in 32 chunks of two groups and 14.4 in 64 of one; 16 of 64 14.3 and 15.0; 128 of 64 54.8 in pairs of CTAs and 56.6
-// in single ones; 256 of 64 102.6 and 107.1; 256 of 16 34.1 and 39.0. The plan was within 4 % of the best of each.
-struct BlocksPlan {
-  int nch;
-  WsGroups groups;
-};
-BlocksPlan plan_blocks(int64_t lists, int k, int n_sm, bool q8) {
-  BlocksPlan best = {1, WsGroups::TWO};
-  double least = 1e300;
-  int last = 0;
-  for (int nch = (k + SEL_CHUNK - 1) / SEL_CHUNK; nch <= std::min(k, std::max(64, (k + SEL_CHUNK - 1) / SEL_CHUNK)); nch++) {
-    const int chunk = (k + nch - 1) / nch;
-    if (chunk == last) continue;  // the same chunks
-    last = chunk;
-    const int64_t ctas = lists * ((k + chunk - 1) / chunk);
-    const double merge = 4e-4 * (double)(ctas * GQA);
-    const double rounds = (double)((ctas + n_sm - 1) / n_sm);
-    const double two = rounds * (5.0 + (q8 ? 0.71 : 1.1) * chunk) + merge;
-    if (two < least) least = two, best = {(k + chunk - 1) / chunk, WsGroups::TWO};
-    if (!q8) continue;
-    const double pairs = (double)((ctas + 2 * n_sm - 1) / (2 * n_sm));
-    const double one = (ctas <= n_sm ? 5.0 + 0.97 * chunk : pairs * (5.0 + 1.37 * chunk)) + merge;
-    if (one < least) least = one, best = {(k + chunk - 1) / chunk, ctas <= n_sm ? WsGroups::SPREAD : WsGroups::PAIRED};
-  }
-  return best;
-}
-
 int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   const CacheRef& c = p.c;
   const int64_t lists = (int64_t)c.B * c.T * c.nkvh, rows = lists * GQA;
   const BlocksPlan plan = plan_blocks(lists, p.k, ctx->n_sm, c.q8);
-  const int nch = plan.nch;
-  const WsGroups groups = plan.groups;
   float* part;
   int64_t fit;
-  if (int rc = place_partials(ctx, p, rows * nch, 0, &fit, &part, who)) return rc;
+  if (int rc = place_partials(ctx, p, rows * plan.nch, 0, &fit, &part, who)) return rc;
   if (fit < rows) return no_room(who);
   const int chunk = (p.k + (int)(fit / rows) - 1) / (int)(fit / rows);
   if (chunk > SEL_CHUNK) return no_room(who);
@@ -366,7 +334,7 @@ int run_blocks(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   if (c.q8) {
     if (int rc = q8_tmaps(p.kcache, cache, &kv, &ks)) return rc;
     if (int rc = q8_tmaps(p.vcache, cache, &vv, &vs)) return rc;
-    if (int rc = launch_blocks_ws(&kv, &ks, &vv, &vs, d, c.B * c.T, s, groups)) return rc;
+    if (int rc = launch_blocks_ws(&kv, &ks, &vv, &vs, d, c.B * c.T, s, plan.pairs)) return rc;
   } else {
     if (int rc = cached_tmap_2d(&kv, p.kcache, cache, 2 * AD, 2 * AD, 128, BLK, true)) return rc;
     if (int rc = cached_tmap_2d(&vv, p.vcache, cache, 2 * AD, 2 * AD, 128, BLK, true)) return rc;

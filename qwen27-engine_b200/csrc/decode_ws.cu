@@ -859,8 +859,7 @@ int smem_of(WsGroups groups) { return groups == WsGroups::SPREAD ? SPREAD_SMEM_B
 
 template <bool PAGED, int NG>
 int blocks_attr() {
-  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, Rows::LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               NG == 1 ? SPREAD_SMEM_BYTES : Lay<NG>::SEL_SMEM_BYTES));
+  Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, Rows::LIST>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<NG>::SEL_SMEM_BYTES));
   if (NG == 1)
     Q27B_CK(cudaFuncSetAttribute(decode_ws_kernel<1, PAGED, NG, Rows::LIST>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
   return Q27B_OK;
@@ -931,7 +930,7 @@ int launch_prefix_ws_paged(const CUtensorMap* kv, const CUtensorMap* ks, const C
 }
 
 int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtensorMap* vv, const CUtensorMap* vs,
-                     const ListParams& p, int nseq, cudaStream_t s, WsGroups groups) {
+                     const ListParams& p, int nseq, cudaStream_t s, bool pairs) {
   static bool attr[64] = {};
   static std::mutex attr_mu;
   int dev;
@@ -948,13 +947,12 @@ int launch_blocks_ws(const CUtensorMap* kv, const CUtensorMap* ks, const CUtenso
   }
   const dim3 grid(p.nch, p.nkvh, nseq);
   const bool paged = p.page_table != nullptr;
-  if (groups == WsGroups::TWO) {
+  if (pairs) {
+    auto* k = paged ? decode_ws_kernel<1, true, 1, Rows::LIST> : decode_ws_kernel<1, false, 1, Rows::LIST>;
+    Q27B_CK(launch_step(k, grid, dim3(Lay<1>::THREADS), Lay<1>::SEL_SMEM_BYTES, s, *kv, *ks, *vv, *vs, p));
+  } else {
     auto* k = paged ? decode_ws_kernel<1, true, 2, Rows::LIST> : decode_ws_kernel<1, false, 2, Rows::LIST>;
     Q27B_CK(launch_step(k, grid, dim3(Lay<2>::THREADS), Lay<2>::SEL_SMEM_BYTES, s, *kv, *ks, *vv, *vs, p));
-  } else {
-    auto* k = paged ? decode_ws_kernel<1, true, 1, Rows::LIST> : decode_ws_kernel<1, false, 1, Rows::LIST>;
-    const int smem = groups == WsGroups::SPREAD ? SPREAD_SMEM_BYTES : Lay<1>::SEL_SMEM_BYTES;
-    Q27B_CK(launch_step(k, grid, dim3(Lay<1>::THREADS), smem, s, *kv, *ks, *vv, *vs, p));
   }
   return Q27B_OK;
 }

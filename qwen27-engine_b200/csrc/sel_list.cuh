@@ -2,6 +2,7 @@
 #pragma once
 #include "common.cuh"
 #include "decode_params.h"
+#include "rows_plan.h"
 
 namespace q27b {
 namespace {
