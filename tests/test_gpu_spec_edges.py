@@ -150,3 +150,212 @@ def test_the_query_counts_outgrown_buffers_and_a_fixed_size_is_exact(q27):
         torch.cuda.synchronize()
         q27.workspace_destroy()
     assert q27.workspace_query() == (0, 0, 0, False)
+
+
+# ---------------------------------------------------------------- every size of the kernels
+def reference_bounds(st, kc, bounds, T):
+    want = bounds.clone()
+    for b, n in enumerate(st.lens):
+        lo, nb = max(0, n - T) // 64, -(-n // 64)
+        if n - T >= n or n <= 0:
+            continue
+        for h in range(st.nkvh):
+            x = st.read(kc, b, h, range(64 * lo, n)).half()
+            at = torch.tensor([H.bounds_at(st, b, h, i) for i in range(lo, nb)], device="cuda")
+            pad = torch.cat([x, x[-1:].expand(64 * (nb - lo) - len(x), -1)]).view(nb - lo, 64, H.AD)
+            want[at, 0], want[at, 1] = pad.amin(1), pad.amax(1)
+    return want
+
+
+@pytest.mark.parametrize("lens,T,nkvh,paged", [
+    ([64 * 460 + 17], 64 * 460 + 17, 4, False), ([64 * 520 + 63], 64 * 470 + 5, 4, False), ([64 * 1900 + 1], 64 * 1800, 1, False),
+    ([8000, 12345, 9001, 8064], 8000, 4, True), ([9000, 100, 7001, 0, 8999, 64], 7001, 4, True)])
+def test_bounds_of_many_blocks(q27, lens, T, nkvh, paged):
+    """From 12 blocks for an SM on a warp takes a block; odd ends, sequences shorter than T, and rows whose scale is NaN."""
+    st = H.Store(lens, T, nkvh, paged, True, seed=T)
+    assert ((T + 62) // 64 + 1) * nkvh * len(lens) >= 12 * torch.cuda.get_device_properties(0).multi_processor_count
+    kc = st.new()
+    st.fill(kc, H.gen(1), 3.0)
+    bounds = H.new_bounds(q27, st, 7.5)
+    want = reference_bounds(st, kc, bounds, T)
+    H.call_bounds(q27, st, kc, bounds, T)
+    assert torch.equal(bounds, want)
+    n = lens[0]
+    st.poison(kc, 0, nkvh - 1, [n - 1, n - 64 * 70])
+    H.call_bounds(q27, st, kc, bounds, T)
+    bad = {H.bounds_at(st, 0, nkvh - 1, p // 64) for p in (n - 1, n - 64 * 70)}
+    nan = torch.isnan(bounds).all(-1).all(-1)
+    assert set(nan.nonzero().flatten().tolist()) == bad and not torch.isnan(bounds[~nan]).any()
+    assert torch.equal(bounds[~nan], want[~nan])
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 2, 3, 4])
+def test_choice_in_a_batch_of_long_and_short_sequences(q27, T):
+    """More groups of 64 blocks than a (KV head, sequence) has CTAs: each goes through several."""
+    r = random.Random(T)
+    lens = [T, 24000, 300 + T, 23999, 64, 16385] + [r.randrange(T, 24000) for _ in range(34)]
+    st = H.Store(lens, T, 4, True, True, seed=T)
+    bounds = H.new_bounds(q27, st)
+    bounds.copy_(torch.randn(bounds.shape, generator=H.gen(T), device="cuda") + torch.tensor([-2.0, 2.0], device="cuda")[:, None])
+    qn, _ = H.queries(st, 3)
+    for k, sink, recent in ((5, 1, 2), (100, 0, 1)):
+        assert torch.equal(H.call_select(q27, st, qn, bounds, k, sink, recent).cpu(), H.select_reference(st, qn, bounds, k, sink, recent))
+    assert q27.device_status() == 0
+
+
+def long_list(nb, k, full, r):
+    """A list of k entries: `full` blocks at its front, the others anywhere behind, -1 between them, and some entries that are none."""
+    blocks = r.sample(range(nb), nb)
+    out = blocks[:full] + [-1] * (k - full)
+    at = r.sample(range(full, k), min(k - full, nb - full) // 2 + (k - full) // 50)
+    for i, x in zip(at, blocks[full:] + [-2, 2 ** 30, -2 ** 31] * k):
+        out[i] = x
+    return out
+
+
+@pytest.mark.parametrize("paged,q8", [(False, True), (False, False), (True, True)])
+@pytest.mark.parametrize("k,full,n,T", [(129, 100, 9000, 4), (1000, 200, 30000, 2), (16384, 128, 30000, 2)])
+def test_lists_of_every_length(q27, paged, q8, k, full, n, T):
+    """Chunks of a list up to the 128 entries that a CTA takes, whole or with blocks far behind each other."""
+    lens = [n, 5000, 64 * full + T] if paged else [n]
+    st = H.Store(lens, T, 2, paged, q8, seed=k)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    r = random.Random(k)
+    sel = torch.tensor([[[long_list((ln - T + t) // 64 + 1, k, min(full, (ln - T + t) // 64 + 1), r) for _ in range(2)] for t in range(T)]
+                        for ln in lens], dtype=torch.int32)
+    qn, qg = H.queries(st, 3)
+
+    def visible(b, t, h):
+        last = st.lens[b] - T + t
+        return [p for x in sel[b, t, h].tolist() if 0 <= x <= last // 64 for p in range(x * 64, min((x + 1) * 64, last + 1))]
+    ref = H.attention(st, kc, vc, qn, qg, visible)
+    o = H.call_blocks(q27, st, kc, vc, qn, qg, sel.cuda())
+    H.check_attention(o, ref)
+    assert q27.device_status() == (4 if ((sel < -1) | (sel == 2 ** 30)).any() else 0)  # entries that are none
+    sel[(sel < 0) | (sel > n // 64)] = -1
+    assert torch.equal(H.call_blocks(q27, st, kc, vc, qn, qg, sel.cuda()), o)
+    assert q27.device_status() == 0
+
+
+def test_many_lists(q27):
+    """Pairs of CTAs on an SM: more chunks than SMs."""
+    T, k, lens = 4, 150, [4000 + 300 * i for i in range(20)]
+    st = H.Store(lens, T, 4, True, True, seed=1)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    r = random.Random(1)
+    sel = torch.tensor([[[sorted(r.sample(range(-(-n // 64)), 50)) + [-1] * (k - 50) for _ in range(4)] for _ in range(T)] for n in lens],
+                       dtype=torch.int32)
+    qn, qg = H.queries(st, 3)
+
+    def visible(b, t, h):
+        last = lens[b] - T + t
+        return [p for x in sel[b, t, h].tolist() if x >= 0 for p in range(x * 64, min((x + 1) * 64, last + 1))]
+    H.check_attention(H.call_blocks(q27, st, kc, vc, qn, qg, sel.cuda()), H.attention(st, kc, vc, qn, qg, visible))
+    assert q27.device_status() == 0
+
+
+def test_long_parts_of_a_batch(q27):
+    """Parts of more than 32 tiles, with and without pages that do not exist in their second half."""
+    T, nkvh, lens = 6, 4, [20000, 12001, 17000, 19937, 3, 16000, 13999, 20000]
+    st = H.Store(lens, T, nkvh, True, True, seed=1)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    masks = H.random_masks(st.B, T, seed=2)
+    qn, qg = H.queries(st, 3)
+    whole = H.tree_visible(st, masks)
+    H.check_attention(H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks)), H.attention(st, kc, vc, qn, qg, whole))
+    assert q27.device_status() == 0
+    bad = {0: {10, 22, 23, 50}, 3: {9, 77}, 6: {40}}  # sequence -> pages of four tiles
+    for b, pages in bad.items():
+        for pg in pages:
+            st.table[b, pg] = -1
+    ref = H.attention(st, kc, vc, qn, qg, lambda b, t, h: [p for p in whole(b, t, h) if p // 256 not in bad.get(b, ())])
+    H.check_attention(H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks)), ref)
+    assert q27.device_status() == 2
+
+
+# ---------------------------------------------------------------- a bound that is not the longest length
+def widen_table(st, pages):
+    more = torch.full((st.B, pages - st.max_pages), -1, dtype=torch.int32, device="cuda")
+    st.table, st.max_pages = torch.cat([st.table, more], 1).contiguous(), pages
+
+
+@pytest.mark.parametrize("T", [1, 4, 5, 20])
+@pytest.mark.parametrize("bound", [200, 700, 1003, 5000, 100000])
+def test_trees_and_the_bound_of_the_lengths(q27, T, bound):
+    """Sequences behind max_seq_len are cut there, drafts among what is cut; a bound far above the lengths changes nothing."""
+    lens = [1000, 150, 730, T, 705]
+    st = H.Store(lens, T, 2, True, True, seed=T)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    widen_table(st, 400)
+    st.max_len = bound
+    masks = H.random_masks(st.B, T, seed=T)
+    qn, qg = H.queries(st, 3)
+    whole = H.tree_visible(st, masks)
+    ref = H.attention(st, kc, vc, qn, qg, lambda b, t, h: [p for p in whole(b, t, h) if p < bound])
+    H.check_attention(H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks)), ref)
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("T", [1, 3])
+@pytest.mark.parametrize("bound", [64, 1000, 1003, 5000, 100000])
+def test_choice_and_the_bound_of_the_lengths(q27, T, bound):
+    lens = [4000, 150, 1500, 64, 1010]
+    st = H.Store(lens, T, 2, True, True, seed=T)
+    bounds = H.new_bounds(q27, st)
+    bounds.copy_(torch.randn(bounds.shape, generator=H.gen(T), device="cuda") + torch.tensor([-2.0, 2.0], device="cuda")[:, None])
+    qn, _ = H.queries(st, 3)
+    want = []
+    for t in range(T):  # a token at position p chooses as the last token of a sequence of min(p + 1, bound) positions
+        one = H.Store([min(n - T + t + 1, bound) for n in lens], 1, 2, True, True, seed=T)
+        one.host_table = st.host_table
+        want.append(H.select_reference(one, qn[:, t:t + 1], bounds, 6, 1, 2))
+    widen_table(st, 400)
+    st.max_len = bound
+    assert torch.equal(H.call_select(q27, st, qn, bounds, 6, 1, 2).cpu(), torch.cat(want, 1))
+    assert q27.device_status() == 0
+
+
+# ---------------------------------------------------------------- scores that cancel
+@pytest.mark.parametrize("T", [1, 2, 4])
+@pytest.mark.parametrize("kind", ["equal", "halves", "mixed", "steps"])
+def test_scores_that_cancel(q27, kind, T):
+    """Scores that are tiny beside the sum A of the products' magnitudes and differ by 2^-12 to 2^-20 of it, at the resolution of the
+    first pass (2^-14 A) and below: a block that its rounded score settled wrongly would show. The products are exact in 64 bits and their sums are
+    off by less than 2^-43 A."""
+    n_blocks, k = 700, 90
+    st = H.Store([64 * n_blocks], T, 2, False, True, seed=1, n_ctx=64 * n_blocks)
+    g = H.gen(T)
+    rnd = lambda *s: torch.rand(s, generator=g, device="cuda")  # noqa: E731
+    sign = lambda *s: torch.where(rnd(*s) < 0.5, -1.0, 1.0)  # noqa: E731
+    for scale in (1.0, 2.0 ** -9, 300.0):
+        bounds = H.new_bounds(q27, st, 0.0)
+        N = bounds.shape[0]
+        if kind == "steps":  # one vector of values, of a few of which the last bit differs; the query's signs cancel its sum
+            x = (1 + rnd(H.AD)).half()
+            v = x.view(torch.int16).repeat(N, 1) + (rnd(N, H.AD) < 0.3).to(torch.int16)
+            v = v.view(torch.float16).float()
+            a = (1 + rnd(H.AD)) * sign(H.AD)
+            a[-1] = -(a[:-1] * x[:-1].float()).sum() / x[-1].float()
+        else:  # the second half takes back what the first gives, but for one dim
+            big = {"equal": torch.ones(N, 1, device="cuda"), "halves": 1 + rnd(N, 1), "mixed": torch.exp2(-8 * rnd(N, 1))}[kind]
+            half = (big * (1 + rnd(N, 128)) * sign(N, 128)).half().float()
+            v = torch.cat([half, half], 1)
+            a = (1 + rnd(128)) * sign(128)
+            a = torch.cat([a, -a])
+            A = 2 * (a[:128].abs() * half.abs()).sum(-1).mean()
+            step = 2.0 ** (-12 - 8 * torch.rand(N, generator=g, device="cuda"))
+            v[:, 5] += A * step * sign(N) / a[5].abs()
+        v = (v * scale).half()
+        bounds[:, 0], bounds[:, 1] = v, v  # (lo = hi: the score is q.v)
+        qn = a.repeat(1, T, st.nqh, 1) * torch.exp2(torch.arange(T * st.nqh, device="cuda") % 5 - 2.0).view(1, T, st.nqh, 1)
+        assert torch.equal(H.call_select(q27, st, qn, bounds, k, 1, 2).cpu(), H.select_reference(st, qn, bounds, k, 1, 2)), scale
+    assert q27.device_status() == 0
