@@ -245,9 +245,12 @@ __device__ __forceinline__ int blocks_of(const CacheRef& c, int b, int t) {
 // lie in memory (a lane's 16 bytes are two k-steps; the order of the dims is free), all of them in registers at once (one token) or half, the
 // query heads are six of the eight columns of B. q times a power of two, so that its largest value is below 2^10, is the sum
 // of two f16 values, off by at most 2^-22 of itself or 2^-25. Four accumulators: q+ hi and q- lo, with the larger parts and with
-// the smaller ones, 16 MMAs each. With A = sum |q| max(|lo|, |hi|) (a fifth one, of |q| + 2^-6), and 17 addends of
-// an MMA each cut at 2^-23 of the largest, the error is below 16 * 18 * 2^-23 A + 2^-22 A < 2^-14.7 A; 2^-14 A is what is
-// passed on. 32 sequences of up to 131,072 positions, two tokens: 45 us for 147 MB of bounds, between the latency of their loads
+// the smaller ones, 16 MMAs each. With A = sum |q| max(|lo|, |hi|) (a fifth one, of |q| + 2^-6): the PTX ISA promises an MMA of f16
+// into f32 products and sums of at least single precision, and what is published of tensor cores (Fasi, Higham, Mikaitis, Pranesh,
+// "Numerical behavior of NVIDIA tensor cores", PeerJ Computer Science 7:e330, 2021) is exact products whose sum with the accumulator
+// is cut at 2^-23 of the largest addend or below. With each of 17 addends cut there the error is below 16 * 18 * 2^-23 A +
+// 2^-22 A < 2^-14.7 A; 2^-14 A is what is passed on. Measured against 64 bits over 45 million sums (signs that cancel, magnitudes
+// of 14 binades, one product among 255 of 2^-24 of it): at most 2^-17.5 A. 32 sequences of up to 131,072 positions, two tokens: 45 us for 147 MB of bounds, between the latency of their loads
 // (a quarter of the issue slots and of the tensor pipe is used; more warps would need the registers that hold loads in flight) and
 // memory; one token behind 150,000 positions: one trip to memory, 4 us.
 constexpr int SCORE_WARPS = 4, SCORE_GROUP = 16 * SCORE_WARPS, Q_STRIDE = 2 * AD + 64;  // bytes between staged query rows: 16-byte reads without conflicts
