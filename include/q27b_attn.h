@@ -22,7 +22,10 @@
  * q27b_attn_workspace_init.
  * Threading: one caller thread per device at a time (as the reference, src/attn.cu:869-879);
  * different devices may be driven from different threads (the process-wide state - tensor-map
- * cache, kernel choices, one-time set-up - is synchronised).
+ * cache, kernel choices, one-time set-up - is synchronised). On the GPU, calls and graphs that use the same part of the
+ * workspace must not overlap, on whichever streams they are: the decode partials (q27b_attn_decode and its kin, trees of up to
+ * four drafts), the prefill partials (q27b_attn_prefill; trees, choices and lists of blocks of one sequence, so a step that
+ * drafts that way must not run beside a prefill), the buffer of the calls over pages. q27b_kv_commit and q27b_kv_bounds use none.
  */
 #ifndef Q27B_ATTN_H_
 #define Q27B_ATTN_H_
@@ -433,8 +436,8 @@ int q27b_prefill_qk_debug(const float* x, int rows, float kq_scale, const void* 
  * q27b_kv_commit moves its rows to the front, q27b_kv_bounds brings the blocks' bounds up to date. A draft step with few
  * blocks: q27b_attn_prep, q27b_kv_bounds, q27b_select_blocks, q27b_attn_decode_blocks.
  * Their scratch lies in the workspace, of one sequence in the prefill buffer (at its fixed size; a smaller one makes for fewer
- * parts, or Q27B_UNSUPPORTED) or, for trees of up to four drafts, in the decode buffer; over pages in the paged buffer. Calls
- * that can overlap on the GPU race on it, so keep those of one device in one stream order. Float and cache pointers lie on
+ * parts, or Q27B_UNSUPPORTED) or, for trees of up to four drafts, in the decode buffer; over pages in the paged buffer (on
+ * overlapping calls see "Threading" above). Float and cache pointers lie on
  * 16-byte boundaries. Indices that the device finds out of range are reported in the device status word (bit 1: page table,
  * bit 2: path or list of blocks) and nothing is read or written there: a path's or list's entry is skipped, and so are the rows
  * of a page (q27b_attn_decode_paged takes those of page 0 in their place). */
@@ -476,7 +479,8 @@ int q27b_kv_commit_paged(void* kpool, void* vpool, const int* page_table, const 
  * [n_pages][nkvh][4][2][256] beside a K pool. The call writes the bounds of every block that holds one of the rows
  * *pos0 .. *pos0 + T - 1 (paged: seq_len[b] - T ..), over all rows of the block below *pos0 + T: after an append, a commit
  * or a prompt's chunk, or of the whole cache at once. NaN in a key makes its bound NaN. Pages that sequences share share their
- * bounds; q27b_kv_page_copy copies none (bring the new page's up to date with this call). */
+ * bounds, so the T rows must lie on pages that no longer sequence shares (what lies behind this one's end would be left out of
+ * them), as appended rows do; q27b_kv_page_copy copies none (bring the new page's up to date with this call). */
 uint64_t q27b_kv_bounds_bytes(int nkvh, int n_ctx);
 uint64_t q27b_kv_bounds_pool_bytes(int nkvh, int n_pages);
 int q27b_kv_bounds(const void* kcache, void* bounds, const int* pos0, int T, int nkvh, int n_ctx, int q8, void* stream);

@@ -2,7 +2,7 @@
 // mask), and T tokens that each attend their own list of 64-position blocks.
 //
 // y = sigmoid(gate) * sum_p P_p v_p with P the softmax of kq_scale * q.k over the visible rows p, in f32; 0 where a row
-// sees nothing. Rows that are not visible are not read, whatever they hold.
+// sees nothing. Rows that are not visible may be loaded (tiles of 64), but have no influence, whatever they hold.
 //
 // The split kernels leave the partials (m, l, O) of a row for every part of its positions; the kernels here merge them. Trees:
 // decode_tree.cu, or for up to four drafts the kernels of q27b_attn_decode over the prefix. Lists of blocks: the split-K kernels
@@ -347,10 +347,11 @@ int run_tree(DeviceCtx* ctx, RowsParams& p, const char* who, cudaStream_t s) {
   const CacheRef& c = p.c;
   if (c.T <= Q27B_MAX_T && c.nkvh <= ctx->n_sm && (c.q8 || (int64_t)c.nkvh * c.n_ctx <= 32768)) {
     // Up to four drafts are 24 rows of a KV head. The decode kernels, made for those, take the prefix, and the merge the drafts:
-    // four behind 1,000 positions 9.2 us against 10.6 with the 128-row tiles of decode_tree.cu, behind 150,000 74 against 98, a
-    // single one 58 against 89; four each behind 16 sequences of up to 16,384 78 against 109, of 64 to 4,096 38 against 44. An f16
-    // cache has nothing to convert there and is bound by its reads earlier: four behind 8,000 positions of four heads 18.4 against
-    // 19.4, behind 16,000 27 against 25, behind 150,000 129 against 106.
+    // four behind 1,000 positions 8.8 us against 9.9 with the 128-row tiles of decode_tree.cu, behind 150,000 70 against 84 (cool), a
+    // single one 58 against 85; four each behind 16 sequences of up to 16,384 80 against 101, of 64 to 4,096 39 against 40. An f16
+    // cache has nothing to convert there and is bound by its reads earlier: four behind 8,000 positions of four heads 13.5 against
+    // 15.2, behind 16,000 17.5 against 18.5, behind 32,000 36 against 32, behind 150,000 137 against 104 (a single one: 16,000 12 against
+    // 18, 150,000 112 against 101). Only the allocated rows are known here; a long cache is taken to be a full one.
     PrefixPartials pre;
     if (c.page_table) {
       if (int rc = launch_prefix_paged(ctx, p.qn, p.kcache, p.vcache, c.page_table, c.seq_len, c.B, c.T, p.kq_scale, c.nkvh, c.n_pages,

@@ -21,8 +21,12 @@
 // memory, which 64 KB of operands a tile written and read again keep busy already, the int8 tile would cost another 68 KB.
 // TMEM: columns 0-255 O (f32), 256-383 two buffers of 64 columns for S (f32) and over it P (f16), 384-511 the Q tile.
 //
-// Measured (events, 16 drafts behind 150,000 positions of four heads, 327 MB and 59 GFLOP): 95 us with the GPU cool, 114 in a long
-// run, in which it draws 970 W and lowers its clock to 1.54 GHz: 2.9 TB/s, 0.52 PFLOP/s. At full clock a tile takes 2,600 cycles of an SM;
+// Drafted V values that are not finite: f16 rows are cleaned by the softmax warps, q8_0 rows by the warp that issues P V, while the
+// softmax is at the tile. (In the converters, whose registers are all taken, a batch of 16 sequences took 124 to 138 us instead of
+// 114; the values added in this kernel's epilogue instead of the merge: 138.)
+//
+// Measured (events, 16 drafts behind 150,000 positions of four heads, 327 MB and 59 GFLOP): 91 to 94 us with the GPU cool, 115 in a long
+// run, in which it draws 970 W and lowers its clock to 1.54 GHz: 2.8 TB/s, 0.51 PFLOP/s. At full clock a tile takes 2,600 cycles of an SM;
 // the MMAs are 1,000 of them, MMAs and softmax without the int8 tiles 1,780 (65 us). The following left it at 93 to 98 us and
 // are not in: the next tiles brought into L2 ahead, int8 tiles through TMA into shared memory two ahead, all loads of a tile in a burst,
 // 32-byte loads, no exponentials, 16 converter warps (101). P in shared memory instead of over S: 98 cool and 117 long, a batch of 16

@@ -34,7 +34,7 @@ struct DeviceCtx {
   // Split partials. Three buffers, so that no call frees what another call's captured graph still
   // names (the reference keeps its prefill buffer apart and fixed for the same reason, src/attn.cu:954-959):
   WsBuf dec;                  // decode of one sequence: n_sm chunk partials, fixed size, allocated on first use
-  WsBuf pf;                   // prefill: allocated once at pf_cap_floats; the split count is cut to fit
+  WsBuf pf;                   // prefill, and trees, choices and lists of blocks of one sequence: allocated once at pf_cap_floats; parts are cut to fit
   GrowingWs paged;            // calls over pages: grows with the batch unless the workspace is frozen
   size_t pf_cap_floats = 0;   // 0: default (see workspace_defaults in host.cu)
   bool frozen = false;        // after q27b_attn_workspace_init: nothing may be allocated any more

@@ -11,7 +11,7 @@ namespace {
 // ---------------------------------------------------------------- commit
 // Row first + i <- row first + path[i] for i < count, K and V, every head. A CTA owns one (head, K or V, sequence): it
 // holds all moved rows in registers (up to 64 rows of 272 or 512 bytes in 256 threads) before it writes the first, so a
-// path may name rows in any order. Launch and latency bound: 16 drafts of one sequence 3.3 us a call, 64 of each of 64 sequences 4.1.
+// path may name rows in any order. Launch and latency bound: 16 drafts of one sequence 3.2 to 3.7 us a call, 64 of each of 64 sequences 4.1.
 constexpr int COMMIT_WARPS = 8, COMMIT_ROWS = MAX_TREE_T / COMMIT_WARPS;
 
 __global__ void __launch_bounds__(32 * COMMIT_WARPS) commit_kernel(const CacheRef c, void* kcache, void* vcache, const int* path,
@@ -68,7 +68,7 @@ int launch_commit(const CacheRef& c, void* kcache, void* vcache, const int* path
 // ---------------------------------------------------------------- bounds
 // Per (block of 64 positions, head, dim) the smallest and the largest key as attention reads it (f16; q8_0: value times
 // scale, rounded once), over the rows of the block below the sequence's end. NaN stays NaN. One CTA a block and head: 16
-// lanes hold a row, 16 row groups take four rows each, all loaded before the first is used. The block of one token: 3.7 us a
+// lanes hold a row, 16 row groups take four rows each, all loaded before the first is used. The block of one token: 3.6 to 4.0 us a
 // call, launch and two trips to memory.
 constexpr int BND_THREADS = 256;
 
