@@ -359,3 +359,152 @@ def test_scores_that_cancel(q27, kind, T):
         qn = a.repeat(1, T, st.nqh, 1) * torch.exp2(torch.arange(T * st.nqh, device="cuda") % 5 - 2.0).view(1, T, st.nqh, 1)
         assert torch.equal(H.call_select(q27, st, qn, bounds, k, 1, 2).cpu(), H.select_reference(st, qn, bounds, k, 1, 2)), scale
     assert q27.device_status() == 0
+
+
+# ---------------------------------------------------------------- shapes and positions at the ends of what is allowed
+@pytest.mark.parametrize("T", [2, 5])
+def test_more_sequences_than_threads(q27, T):
+    r = random.Random(T)
+    lens = [r.choice([0, 1, T, 64, 70]) for _ in range(1300)]
+    st = H.Store(lens, T, 1, True, True, seed=T)
+    kc, vc = st.new(), st.new()
+    g = H.gen(1)
+    for buf in (kc, vc):
+        v, s = st.parts(buf)
+        v.copy_(torch.randint(-127, 128, v.shape, generator=g, device="cuda", dtype=torch.int8))
+        s.copy_(torch.rand(s.shape, generator=g, device="cuda") * 0.02)
+    masks = H.random_masks(st.B, T, seed=T)
+    qn, qg = H.queries(st, 3)
+    o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+    H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("nkvh,n_ctx", [(7, 131), (16, 200), (149, 70), (200, 65)])
+@pytest.mark.parametrize("q8", [True, False])
+def test_many_heads(q27, nkvh, n_ctx, q8):
+    """More KV heads than SMs among them: trees, their commit, bounds, choice and lists."""
+    for T in (2, 6):
+        n = n_ctx - 3
+        st = H.Store([n], T, nkvh, False, q8, seed=T, n_ctx=n_ctx)
+        kc, vc = st.new(), st.new()
+        st.fill(kc, H.gen(1))
+        st.fill(vc, H.gen(2))
+        masks = H.random_masks(1, T, seed=T)
+        qn, qg = H.queries(st, 3)
+        o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+        H.check_attention(o, H.attention(st, kc, vc, qn, qg, H.tree_visible(st, masks)))
+        if T == 2:
+            bounds = H.new_bounds(q27, st, 7.5)
+            want = reference_bounds(st, kc, bounds, n)
+            H.call_bounds(q27, st, kc, bounds, n)
+            assert torch.equal(bounds, want)
+            sel = H.call_select(q27, st, qn, bounds, 2, 0, 1)
+            ref = H.select_reference(st, qn, bounds, 2, 0, 1)
+            assert torch.equal(sel.cpu(), ref)
+            seen = lambda b, t, h: [p for x in ref[b, t, h].tolist() if x >= 0 for p in range(64 * x, min(64 * x + 64, n - T + t + 1))]  # noqa: E731
+            H.check_attention(H.call_blocks(q27, st, kc, vc, qn, qg, sel), H.attention(st, kc, vc, qn, qg, seen))
+        k0, v0 = kc.clone(), vc.clone()
+        q27.kv_commit(kc, vc, st.pos0, H.i32([T - 1] + [0] * (T - 1)), H.i32([1]), T, nkvh, n_ctx, q8)
+        for new, old in ((kc, k0), (vc, v0)):
+            (a, sa), (b, sb) = st.parts(new), st.parts(old)
+            at = torch.tensor([int(st.index(0, h, [n - T])) for h in range(nkvh)], device="cuda")
+            b[at] = b[at + T - 1]
+            if sb is not None:
+                sb[at] = sb[at + T - 1]
+            assert torch.equal(new, old)
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("q8", [True, False])
+@pytest.mark.parametrize("T", [3, 9])
+def test_drafts_outside_the_cache(q27, T, q8):
+    """Positions before the cache and behind it: what lies inside is attended, the rest is not there."""
+    n_ctx = 150
+    for pos in (-T, 1 - T, -1, n_ctx - T, n_ctx - T + 1, n_ctx - 1, n_ctx, n_ctx + 70):
+        st = H.Store([n_ctx], T, 2, False, q8, seed=T, n_ctx=n_ctx)
+        kc, vc = st.new(), st.new()
+        st.fill(kc, H.gen(1))
+        st.fill(vc, H.gen(2))
+        masks = H.random_masks(1, T, seed=T, empty=False)
+        qn, qg = H.queries(st, 3)
+        st.pos0.fill_(pos)
+
+        def seen(b, t, h):
+            return [p for p in range(n_ctx) if p < pos] + [pos + j for j in range(T) if 0 <= pos + j < n_ctx and (masks[0][t] >> j) & 1]
+        o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+        H.check_attention(o, H.attention(st, kc, vc, qn, qg, seen))
+        if T == 3:
+            sel = torch.arange(3, dtype=torch.int32, device="cuda").expand(1, T, 2, 3).contiguous()
+            o = H.call_blocks(q27, st, kc, vc, qn, qg, sel)
+            H.check_attention(o, H.attention(st, kc, vc, qn, qg, lambda b, t, h: list(range(max(0, min(n_ctx, pos + t + 1))))))
+            bounds = H.new_bounds(q27, st, 0.0)
+            got = H.call_select(q27, st, qn, bounds, 4, 1, 1)[0, :, 0].tolist()
+            nb = [max(0, min(n_ctx - 1, pos + t) // 64 + 1) if pos + t >= 0 else 0 for t in range(T)]
+            assert got == [list(range(x)) + [-1] * (4 - x) for x in nb]
+    assert q27.device_status() == 0
+
+
+@pytest.mark.parametrize("paged,q8,n_ctx", FORMS)
+@pytest.mark.parametrize("T", [4, 7])
+def test_a_query_that_is_not_finite_stays_in_its_row(q27, T, paged, q8, n_ctx):
+    st = H.Store([500], T, 2, paged, q8, seed=T, n_ctx=n_ctx)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    masks = H.random_masks(1, T, seed=T)
+    qn, qg = H.queries(st, 3)
+    clean = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+    qn[0, 1, 3, 17], qn[0, 2, 8, 200] = math.nan, math.inf
+    o = H.call_tree(q27, st, kc, vc, qn, qg, H.mask_tensor(masks))
+    rows = torch.ones(o.shape[:3], dtype=torch.bool, device="cuda")
+    rows[0, 1, 3] = rows[0, 2, 8] = False
+    assert torch.isnan(o[0, 1, 3]).all() and torch.equal(o[rows], clean[rows])
+    assert q27.device_status() == 0
+
+
+def test_bookkeeping_over_pages_that_do_not_exist(q27):
+    """Commit leaves rows whose source or destination is on no page, bounds leave such blocks, the choice ranks them last."""
+    T, nkvh, lens = 6, 2, [600, 515, 3000]
+    st = H.Store(lens, T, nkvh, True, True, seed=1)
+    kc, vc = st.new(), st.new()
+    st.fill(kc, H.gen(1))
+    st.fill(vc, H.gen(2))
+    good = st.table.clone()
+    st.table[1, 2] = st.n_pages  # positions 512 .. of the second sequence: drafts 509 .. 514
+    before = kc.clone(), vc.clone()
+    path = [[5, 4, 3, 2, 1, 0]] * 3
+    q27.kv_commit_paged(kc, vc, st.table, st.seq_len, H.i32(path), H.i32([6, 6, 0]), 3, T, nkvh, st.n_pages, st.max_pages)
+    assert q27.device_status() == 2
+    st.table.copy_(good)
+    for new, old in zip((kc, vc), before):
+        for h in range(nkvh):
+            assert torch.equal(st.read(new, 0, h, range(594, 600)), st.read(old, 0, h, range(594, 600)).flip(0))
+            assert torch.equal(st.read(new, 1, h, range(515)), st.read(old, 1, h, range(515)))
+            assert torch.equal(st.read(new, 2, h, range(3000)), st.read(old, 2, h, range(3000)))
+    bounds = H.new_bounds(q27, st, 7.5)
+    want = reference_bounds(st, kc, bounds, 600)
+    bad = {0: [1], 1: [2], 2: [10, 11]}
+    for b, pages in bad.items():
+        for pg in pages:
+            st.table[b, pg] = -3
+            for h in range(nkvh):
+                for blk in range(4 * pg, 4 * pg + 4):
+                    want[H.bounds_at(st, b, h, blk)] = 7.5
+    H.call_bounds(q27, st, kc, bounds, 600)
+    assert q27.device_status() == 2 and torch.equal(bounds, want)
+    # the choice: every key is small, what the bad pages' bounds say (7.5) would win
+    H.call_bounds(q27, st, kc, bounds, 3000)
+    q27.device_status()
+    st.T, one = 1, H.Store(lens, 1, nkvh, True, True, seed=1)
+    qn, _ = H.queries(one, 3)
+    sel = H.call_select(q27, st, qn, bounds, 8, 0, 1)
+    assert q27.device_status() == 2
+    for b, n in enumerate(lens):
+        nb = (n - 1) // 64 + 1
+        for h in range(nkvh):
+            got = [x for x in sel[b, 0, h].tolist() if x >= 0]
+            gone = [x for x in range(nb - 1) if x // 4 in bad[b]]
+            assert got == sorted(got) and len(got) == min(8, nb) and got[-1] == nb - 1
+            there = nb - len(gone)
+            assert len([x for x in got if x in gone]) == max(0, min(8, nb) - there)
